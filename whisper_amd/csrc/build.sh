@@ -4,7 +4,8 @@ set -e
 cd "$(dirname "$0")"
 JOBS=4
 [ "$1" = "-j" ] && JOBS=$2
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function"
+# no packed-fp32 instructions: some of their forms have given wrong results on this hardware now and then
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _build
 pids=()
 for f in uw_api uw_gemm uw_elementwise uw_attention uw_decode uw_mel uw_align; do

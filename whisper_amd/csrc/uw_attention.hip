@@ -185,8 +185,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             const float m_new = fmaxf(m_run, mx);
             const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * LOG2E);  // first tile: exp2(-inf) = 0
             const float neg_m = -m_new * LOG2E;
-            // two scores per instruction for the scale-and-shift and for the row sum (v_pk_fma_f32 / v_pk_add_f32): the
-            // vector ALU, not the matrix pipe, is what this loop keeps busiest
+            // scores in pairs for the scale-and-shift and for the row sum: the vector ALU, not the matrix pipe, is what this
+            // loop keeps busiest (the build excludes the packed instructions these pairs would otherwise become)
             typedef __attribute__((ext_vector_type(2))) float f32x2;
             const f32x2 l2e = {LOG2E, LOG2E}, nm2 = {neg_m, neg_m};
             f32x2 rs2 = {0.f, 0.f};
