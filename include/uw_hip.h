@@ -159,6 +159,74 @@ int uw_profile_end(uw_ctx* ctx, int64_t* launches_total, int64_t* launches_timed
  * uw_profile_end: how many ran, how many were timed, the summed duration of the timed ones. */
 int uw_profile_span(uw_ctx* ctx, int kind, int64_t* launches_total, int64_t* launches_timed, double* timed_ms);
 
+/* ---- 8-bit paged key/value cache and draft verification -------------------------------------------------------------
+ * Context-free operators for serving (no counterpart in the reference, which feeds its past_key_values.* empty,
+ * core.py:185-192).  They work on the CURRENT device, allocate nothing, never synchronise and may be captured into a graph.
+ *
+ * The cache is four arrays the caller owns.  A page ("block") holds `page` tokens of all kv heads:
+ *   k        8-bit codes [n_pages][n_kv_heads][page][head_dim]
+ *   v        8-bit codes [n_pages][n_kv_heads][head_dim][page]   (transposed inside the page)
+ *   k_scale, v_scale  f32 [n_pages][n_kv_heads];   value = code * scale
+ * Formats: UW_KV8_INT8 (codes -127..127) and UW_KV8_E4M3 (1-4-3 without infinities, scales are powers of two).  page: 16, 32,
+ * 64, 128 or 256; head_dim: 64 or 128.  k and v must be 16-byte aligned.
+ * table i32 [B][table_width]: the page of each block of a sequence, block i holding positions i * page ... Entries behind a
+ * sequence's end are not read.  A page id outside 0..n_pages-1, or a position behind the table, is never accessed: an append
+ * skips it, a read and an attention row that sees it give NaN.
+ * Tokens come either T per sequence (tok_start NULL, T > 0, n_tok = B * T), sequence b's first row at b * seq_stride, or packed
+ * one sequence behind the other (tok_start i32 [B+1], row r at r * tok_stride; T and seq_stride are ignored); rows behind
+ * tok_start[B] are neither read nor written.  Strides are in elements; element (row, head, i) lies at row + head * head_stride + i;
+ * base pointers and strides must be multiples of 16 bytes.  dtype: UW_DTYPE_F32 or UW_DTYPE_BF16. */
+#define UW_KV8_INT8 0
+#define UW_KV8_E4M3 1
+typedef struct uw_kv8_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t n_pages, n_kv_heads, page, head_dim, format;
+} uw_kv8_cache;
+typedef struct uw_kv8_tokens {      /* a [rows][heads][head_dim] array and how its rows belong to the sequences */
+    void* data;
+    int64_t seq_stride, tok_stride, head_stride;
+    int64_t n_tok;
+    const int32_t* tok_start;
+    int32_t B, T;
+} uw_kv8_tokens;
+
+/* Appends keys and values: sequence b's tokens go to positions pos[b], pos[b] + 1, ... (pos i32 [B] = tokens already there).
+ * Per touched block, head and half: a block without earlier tokens takes its scale from the largest |x|; otherwise the scale
+ * stays while the new values fit and grows by a power of two if not, the earlier tokens' codes being re-rounded.  A NaN or
+ * infinity makes the scale of its block and head NaN until the block is begun again: whatever reads that block gives NaN.
+ * A block of two sequences of one call must not be touched by both (shared prefixes end on a page boundary).  Codes behind the
+ * last token are left as they are.  k->tok_start, B, T and n_tok hold for v too. */
+int uw_kv8_append(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, const uw_kv8_tokens* v, const int32_t* table,
+                  int table_width, const int32_t* pos, void* stream);
+/* Reads tokens back as values (code * scale, rounded once to dtype): positions first[b], first[b] + 1, ... into k and v. */
+int uw_kv8_read(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, const uw_kv8_tokens* v, const int32_t* table,
+                int table_width, const int32_t* first, void* stream);
+/* Attention of n_heads query heads (a multiple of n_kv_heads; query head h reads kv head h / (n_heads / n_kv_heads)) over the
+ * first kv_len[b] cached tokens; with causal != 0 token t of the n tokens of a sequence sees keys 0 .. kv_len[b] - n + t (its
+ * own key, appended before, is the last).  o: rows like q; lse (may be NULL) f32 [n_tok][n_heads]: log of the sum of exp(scores).
+ * A row that sees no key gives 0 and lse = -inf.  scale multiplies q.k.  ws: uw_kv8_attention_workspace_bytes() bytes, 16-byte
+ * aligned, not shared by calls that may run at the same time; NULL if that is 0. */
+int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_cache* cache, int n_heads, int B, int64_t n_tok, int T, int table_width);
+int uw_kv8_attention(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* q, const uw_kv8_tokens* o, float* lse, int n_heads,
+                     const int32_t* table, int table_width, const int32_t* kv_len, int causal, float scale, void* ws,
+                     void* stream);
+
+/* Verification of drafted tokens (speculative decoding): target [B][N+1][V] and draft [B][N][V] (NULL: the drafter is taken to
+ * have been certain of its token) are logits, or probabilities if `probs`; rows at b * *_sB + i * *_sN, elements contiguous.
+ * drafted i32 [B][N], n_drafted i32 [B] (NULL: N for all; clamped to 0..N), uniforms f32 [B][N+1] in [0, 1).
+ * With p_i, q_i = softmax(row / temperature): token i is accepted while uniforms[b][i] * q_i(d_i) < p_i(d_i).  At the first
+ * rejection the next token is drawn from max(p_i - q_i, 0), after the last accepted one from p_n: the smallest index whose
+ * cumulative weight exceeds uniforms[b][N] times the whole.  All of this in 64 bits.  temperature 0: a token is accepted while it
+ * is its row's arg-max (the lowest index of equal ones) and the next token is the arg-max; draft and uniforms are not read.
+ * accepted i32 [B]; tokens i32 [B][N+1]: the accepted tokens, the next token, then -1.  The next token is -1 if its row holds
+ * a NaN or has no mass (the decoder-run failure of core.py:948-956); a drafted id outside 0..V-1 is never accepted.
+ * ws: uw_verify_draft_workspace_bytes() bytes, 16-byte aligned, not shared by calls that may run at the same time. */
+int64_t uw_verify_draft_workspace_bytes(int B, int N, int V);
+int uw_verify_draft(int dtype, const void* target, int64_t target_sB, int64_t target_sN, const void* draft, int64_t draft_sB,
+                    int64_t draft_sN, const int32_t* drafted, const int32_t* n_drafted, const float* uniforms, int B, int N, int V,
+                    float temperature, int probs, int32_t* accepted, int32_t* tokens, void* ws, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
