@@ -127,71 +127,357 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8View c, TokSpan ts, To
     }
 }
 
-// attention, one workgroup per query row and head: 256 keys per round, a lane scores one key; then a lane owns one output element
-template <int F, typename T>
-__global__ __launch_bounds__(256) void kv8_attention_kernel(Kv8View c, TokSpan ts, TokArg qa, TokArg oa, float* lse, int H,
-                                                            const int32_t* kv_len, int causal, float scale)
+// ------------------------------------------------------------------------------------------------
+// Attention.  Rows of one kv head are its G query heads of every query token, token-major: row = t * G + g.  A wave works on 64
+// keys at a time and 16 * RT rows, in registers throughout:
+//   S^T = K Q^T    16x16x32 MFMA, A = K codes as bf16 (exact), B = Q; lane (row = lane & 15, g = lane >> 4) gets for tile t the keys
+//                  16 g + 4 t + 0..3, because row slot r of tile t holds key 16 (r >> 2) + 4 t + (r & 3)
+//   O^T = V^T P^T  A = V codes as they lie (16 consecutive keys 16 g .. of one channel), B = P straight from those lanes
+// so neither K nor V nor P passes through LDS.  Scales multiply the scores (K) and the probabilities (V) -- one per 16 keys at
+// least, so one per lane.  Running maximum, sum and output in f32.  f32 queries and probabilities enter as three bf16 planes (24
+// bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.  bf16 queries are exact; their probabilities are
+// rounded to bf16 (2^-9 of each, independently), which is what the output is rounded to anyway.
+struct AttnArgs {
+    Kv8View c;
+    TokSpan ts;
+    TokArg q, o;
+    float* lse;
+    const int32_t* kv_len;
+    float* part;         // [rows][H][n_split][D + 4] partial results (output, maximum, sum) when n_split > 1
+    int H, G, causal, n_split;
+    int tiles;           // workgroups per sequence (uniform)
+    int lds_rows;        // rows of a tile that can be in use
+    float scale2;        // scale * log2(e)
+};
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+// 8 codes -> an MFMA operand chunk
+template <int F> __device__ __forceinline__ bf16x8 codes8(unsigned a, unsigned b);
+template <> __device__ __forceinline__ bf16x8 codes8<UW_KV8_E4M3>(unsigned a, unsigned b)
 {
-    __shared__ float q[128], p_s[256], red[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.y, D = c.D;
-    const long row = blockIdx.x;
-    int b = 0, t = 0;
-    if (ts.tok_start) {
-        for (int i = 0; i < ts.B; ++i)
-            if (ts.count(i) > 0 && row >= ts.tok_start[i] && row < ts.tok_start[i + 1]) { b = i; t = (int)(row - ts.tok_start[i]) + 1; }
-        if (!t) return;
-        --t;
-    } else {
-        b = (int)(row / ts.T);
-        t = (int)(row % ts.T);
+    union { bf16x2 p[4]; bf16x8 v; } u;
+    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+    return u.v;
+}
+template <> __device__ __forceinline__ bf16x8 codes8<UW_KV8_INT8>(unsigned a, unsigned b)
+{
+    bf16x8 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = (__bf16)(float)(int8_t)(a >> (8 * i));
+        v[4 + i] = (__bf16)(float)(int8_t)(b >> (8 * i));
     }
-    const int g = h / (H / c.Hkv);
-    const long base = ts.tok_start ? row * qa.sT : (long)b * qa.sB + (long)t * qa.sT;
-    const long obase = ts.tok_start ? row * oa.sT : (long)b * oa.sB + (long)t * oa.sT;
-    const long n_keys = causal ? max(0l, (long)kv_len[b] - ts.count(b) + t + 1) : max(0, kv_len[b]);
-    if (tid < D) q[tid] = ld_elem<T>(qa.data, base + h * qa.sH + tid) * scale;
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (long k0 = 0; k0 < n_keys; k0 += 256) {
-        __syncthreads();
-        const long j = k0 + tid;
-        float s = -INFINITY;
-        if (j < n_keys) {
-            const int page = kv8_page(c, b, j >> c.log2P);
-            const long at = (long)max(page, 0) * c.Hkv + g;
-            const uint8_t* kr = c.k + (at * c.P + (j & (c.P - 1))) * D;
-            s = 0.f;
-            for (int d = 0; d < D; ++d) s = fmaf(q[d], kv8_decode<F>(kr[d]), s);
-            s = page < 0 ? __uint_as_float(0x7fc00000u) : s * c.ks[at];
+    return v;
+}
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// the planes of 8 f32 values
+template <int NP> __device__ __forceinline__ void planes(const float* x, bf16x8* out)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float rest = x[e];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const __bf16 part = (__bf16)rest;
+            out[n][e] = part;
+            rest -= (float)part;
         }
-        const bool bad = __syncthreads_or(s != s);
-        float mx = wave_max(s);
-        if (lane == 0) red[wave] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        float mn = fmaxf(m, mx);
-        if (bad) mn = __uint_as_float(0x7fc00000u);
-        const float p = (j < n_keys) ? expf(s - mn) : 0.f;
-        const float sum = wave_sum(p);
-        __syncthreads();
-        if (lane == 0) red[wave] = sum;
-        p_s[tid] = p;
-        __syncthreads();
-        const float f = m == -INFINITY ? 0.f : expf(m - mn);
-        l = l * f + ((red[0] + red[1]) + (red[2] + red[3]));
-        acc *= f;
-        m = mn;
-        if (tid < D) {
-            const int lim = (int)min(256l, n_keys - k0);
-            for (int i = 0; i < lim; ++i) {
-                const long jj = k0 + i;
-                const int page = kv8_page(c, b, jj >> c.log2P);
-                const long at = (long)max(page, 0) * c.Hkv + g;
-                acc = fmaf(p_s[i] * c.vs[at], kv8_decode<F>(c.v[(at * D + tid) * c.P + (jj & (c.P - 1))]), acc);
+    }
+}
+
+// keeps the first n of 16 bytes
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int n)
+{
+    auto m = [&](int k) { return k <= 0 ? 0u : k >= 4 ? ~0u : (1u << (8 * k)) - 1u; };
+    return make_uint4(v.x & m(n), v.y & m(n - 4), v.z & m(n - 8), v.w & m(n - 12));
+}
+
+// four channels of a finished row (or of a split's part of it)
+template <typename T, int D>
+__device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first, int kvh, int row, int d, int split, float M, float L, f32x4 acc)
+{
+    const int t = row / p.G, h = kvh * p.G + row % p.G;
+    const long rg = t_first + t;                        // row of the call
+    if (p.n_split > 1) {
+        float* at = p.part + ((rg * p.H + h) * p.n_split + split) * (D + 4);
+        *(f32x4*)(at + d) = acc;
+        if (d == 0) { at[D] = M; at[D + 1] = L; }
+        return;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    T* out = (T*)p.o.data + (p.ts.tok_start ? rg * p.o.sT : (long)b * p.o.sB + (long)t * p.o.sT) + (long)h * p.o.sH + d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(acc[k] * inv);
+    if (p.lse && d == 0) p.lse[rg * p.H + h] = L == 0.f ? -INFINITY : M * LN2 + logf(L);
+}
+
+// WK waves share the keys of a row tile (their results are joined in LDS), WR row tiles per workgroup
+template <int F, typename T, int D, int RT, int WK, int WR>
+__global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
+{
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave % WK, wr = wave / WK;
+    const int rr = lane & 15, g4 = lane >> 4;
+    const Kv8View& c = p.c;
+
+    // which sequence, kv head, rows
+    int b, tile;
+    const int kvh = blockIdx.y, split = blockIdx.z;
+    if (p.ts.tok_start) {
+        if (!locate(blockIdx.x, p.ts.B, [&](int i) { return (int)(((long)p.ts.count(i) * p.G + ROWS * WR - 1) / (ROWS * WR)); }, b, tile)) return;
+    } else {
+        b = blockIdx.x / p.tiles;
+        tile = blockIdx.x % p.tiles;
+    }
+    const int n = p.ts.count(b), n_rows = n * p.G;
+    const int row0 = (tile * WR + wr) * ROWS;
+    const int len = max(0, p.kv_len[b]);
+    const long t_first = p.ts.first(b);
+
+    // keys each of this lane's rows sees; the fewest and the most of the wave's
+    const int row_end = min(row0 + ROWS, n_rows);
+    auto seen = [&](int row) { return p.causal ? max(0, len - n + 1 + row / p.G) : len; };
+    int lim[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) lim[i] = seen(min(row0 + 16 * i + rr, n_rows - 1));
+    const int lim_min = row0 < n_rows ? seen(row0) : 0, lim_max = row0 < n_rows ? seen(row_end - 1) : 0;
+
+    // Q fragments
+    bf16x8 qf[RT][HALF][2][NP];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int row = row0 + 16 * i + rr;
+        const int t = row / p.G, h = kvh * p.G + row % p.G;
+        const long at = (p.ts.tok_start ? (t_first + t) * p.q.sT : (long)b * p.q.sB + (long)t * p.q.sT) + (long)h * p.q.sH + g4 * 16;
+#pragma unroll
+        for (int hf = 0; hf < HALF; ++hf)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if constexpr (NP == 1) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (row < n_rows) w = *(const uint4*)((const T*)p.q.data + at + hf * 64 + s * 8);
+                    qf[i][hf][s][0] = __builtin_bit_cast(bf16x8, w);
+                } else {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = row < n_rows ? to_f32<T>(((const T*)p.q.data)[at + hf * 64 + s * 8 + e]) : 0.f;
+                    planes<NP>(x, qf[i][hf][s]);
+                }
+            }
+    }
+
+    f32x4 o[RT][D / 16];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[i][d] = f32x4{0, 0, 0, 0};
+    }
+
+    // blocks of 64 keys of this split, dealt to the waves
+    const int blocks = (lim_max >> 6) + ((lim_max & 63) ? 1 : 0);
+    const int per = (blocks + p.n_split - 1) / p.n_split;
+    const int blk1 = min(blocks, (split + 1) * per);
+    const long page_bytes = (long)c.P * D;
+    const bool small = c.P < 64;
+    const int k_group = rr >> 2, k_in = rr & 3;     // 16-key group and place in it of this lane's K rows
+    for (int blk = split * per + wk; blk < blk1; blk += WK) {
+        const int j0 = blk << 6, jk = j0 + 16 * k_group, jv = j0 + 16 * g4;
+        int pk, pv;
+        if (small) {
+            pk = kv8_page(c, b, jk >> c.log2P);
+            pv = kv8_page(c, b, jv >> c.log2P);
+        } else {
+            pk = pv = kv8_page(c, b, j0 >> c.log2P);
+        }
+        const uint8_t* kp = c.k + ((long)max(pk, 0) * c.Hkv + kvh) * page_bytes + ((jk & (c.P - 1)) + k_in) * D + g4 * 16;
+        const uint8_t* vp = c.v + ((long)max(pv, 0) * c.Hkv + kvh) * page_bytes + (long)rr * c.P + (jv & (c.P - 1));
+        uint4 kf[4][HALF], vf[D / 16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = *(const uint4*)(kp + t * 4 * D + hf * 64);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) vf[d] = *(const uint4*)(vp + (long)d * 16 * c.P);
+        const float nan = __uint_as_float(0x7fc00000u);
+        const float ks = pv < 0 ? nan : c.ks[(long)pv * c.Hkv + kvh] * p.scale2;
+        const float vs = pv < 0 ? nan : c.vs[(long)pv * c.Hkv + kvh];
+        const bool mask = lim_min - j0 < 64;
+
+        f32x4 st[RT][4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) st[i][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int hf = 0; hf < HALF; ++hf) {
+                const bf16x8 a0 = codes8<F>(kf[t][hf].x, kf[t][hf].y), a1 = codes8<F>(kf[t][hf].z, kf[t][hf].w);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int pl = NP - 1; pl >= 0; --pl) {
+                        st[i][t] = mfma(a0, qf[i][hf][0][pl], st[i][t]);
+                        st[i][t] = mfma(a1, qf[i][hf][1][pl], st[i][t]);
+                    }
+            }
+        bf16x8 pf[RT][2][NP];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    st[i][t][e] *= ks;
+                }
+            const int left = lim[i] - jv;          // keys of this lane's 16 that the row sees
+            if (mask) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (4 * t + e >= left) st[i][t][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[i][t][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m[i], mx);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
+            if (__any(mn != m[i])) {
+                l[i] *= alpha;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) o[i][d] *= alpha;
+            }
+            m[i] = mn;
+            float x[16];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float pr = __builtin_amdgcn_exp2f(st[i][t][e] - base);
+                    l[i] += pr;
+                    x[4 * t + e] = pr * vs;
+                }
+            if (mask) {                            // a scale behind the end may be NaN
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (k >= left) x[k] = 0.f;
+            }
+            planes<NP>(x, pf[i][0]);
+            planes<NP>(x + 8, pf[i][1]);
+        }
+        if (mask) {      // leftovers behind the sequence's end may hold NaN, which a probability of 0 does not silence
+            const int keep = max(0, min(16, len - jv));
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) vf[d] = first_bytes(vf[d], keep);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            const bf16x8 a0 = codes8<F>(vf[d].x, vf[d].y), a1 = codes8<F>(vf[d].z, vf[d].w);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int pl = NP - 1; pl >= 0; --pl) {
+                    o[i][d] = mfma(a0, pf[i][0][pl], o[i][d]);
+                    o[i][d] = mfma(a1, pf[i][1][pl], o[i][d]);
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        l[i] += __shfl_xor(l[i], 16, 64);
+        l[i] += __shfl_xor(l[i], 32, 64);
+    }
+
+    // join the waves that shared the keys
+    if constexpr (WK > 1) {
+        const int R = p.lds_rows;
+        float* sm = lds + (long)wr * WK * R * (D + 2);                    // [WK][R] m, [WK][R] l, [WK][R][D]
+        float* sl = sm + WK * R;
+        float* so = sl + WK * R;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int r = 16 * i + rr;
+            if (r >= R) continue;
+            if (g4 == 0) { sm[wk * R + r] = m[i]; sl[wk * R + r] = l[i]; }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                float* at = so + ((long)wk * R + r) * D + d * 16 + g4 * 4;
+                at[0] = o[i][d][0]; at[1] = o[i][d][1]; at[2] = o[i][d][2]; at[3] = o[i][d][3];
             }
         }
+        __syncthreads();
+        for (int e = (wk * 64 + lane) * 4; e < (row_end - row0) * D; e += 64 * WK * 4) {
+            const int r = e / D, d = e % D;
+            float M = -INFINITY, L = 0.f;
+            f32x4 acc = {0, 0, 0, 0};
+            for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[w * R + r]);
+            for (int w = 0; w < WK; ++w) {
+                // a wave without a finite score has a sum of 0, or NaN where it met a NaN
+                const float mw = sm[w * R + r], f = mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - M);
+                L += sl[w * R + r] * f;
+                const float* x = so + ((long)w * R + r) * D + d;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] += x[k] * f;
+            }
+            store_row<T, D>(p, b, t_first, kvh, row0 + r, d, split, M, L, acc);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int row = row0 + 16 * i + rr;
+            if (row < n_rows)
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) store_row<T, D>(p, b, t_first, kvh, row, d * 16 + g4 * 4, split, m[i], l[i], o[i][d]);
+        }
     }
-    if (tid < D) ((T*)oa.data)[obase + h * oa.sH + tid] = from_f32<T>(n_keys > 0 ? acc / l : 0.f);
-    if (lse && tid == 0) lse[row * H + h] = n_keys > 0 ? m + logf(l) : -INFINITY;
+}
+
+// joins the splits: a wave per (token, head)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p)
+{
+    const int lane = threadIdx.x & 63;
+    const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6), row = w / p.H;
+    const int h = (int)(w % p.H);
+    if (row >= p.ts.N) return;
+    long oat = row * p.o.sT;
+    if (p.ts.tok_start) {
+        if (row < p.ts.tok_start[0] || row >= p.ts.tok_start[p.ts.B]) return;
+    } else {
+        oat = row / p.ts.T * p.o.sB + row % p.ts.T * p.o.sT;
+    }
+    const float* part = p.part + w * p.n_split * (D + 4);
+    float M = -INFINITY, L = 0.f, acc[D / 64] = {};
+    for (int s = 0; s < p.n_split; ++s) M = fmaxf(M, part[s * (D + 4) + D]);
+    for (int s = 0; s < p.n_split; ++s) {
+        const float* x = part + s * (D + 4);
+        const float ms = x[D], ls = x[D + 1];
+        const float f = ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms - M);
+        L += ls * f;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) acc[k] += x[k * 64 + lane] * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) ((T*)p.o.data)[oat + (long)h * p.o.sH + k * 64 + lane] = from_f32<T>(acc[k] * inv);
+    if (p.lse && lane == 0) p.lse[row * p.H + h] = L == 0.f ? -INFINITY : M * LN2 + logf(L);
 }
 
 // ---- host side --------------------------------------------------------------------------------------
@@ -273,6 +559,60 @@ long touched_bound(const uw_kv8_tokens* t, int P)
         }                                                                                   \
     } while (0)
 
+struct AttnPlan {
+    int rt, wk, wr;      // row tiles of 16 per wave, waves sharing keys, waves side by side on rows
+    int n_split, tiles, lds_rows;
+    long groups;         // grid.x
+};
+
+// How a call is cut.  Few rows per sequence: the waves of a workgroup share the keys, and the keys are cut over workgroups until
+// the chip is full.  Many rows: the waves take rows of their own.
+AttnPlan plan_attention(const uw_kv8_cache* c, int n_heads, int B, int64_t n_tok, int T, int width)
+{
+    AttnPlan p;
+    const int G = n_heads / c->n_kv_heads;
+    const long rows = T > 0 ? (long)T * G : (long)ceil_div(n_tok, B) * G;     // per sequence; packed: on average
+    const int max_rt = 2;
+    if (rows <= 16 * max_rt * 2) {
+        p.rt = rows <= 16 ? 1 : 2;
+        p.wk = 4;
+        p.wr = 1;
+    } else {
+        p.rt = 2;
+        p.wk = 1;
+        p.wr = 4;
+    }
+    const int per = 16 * p.rt * p.wr;
+    p.lds_rows = T > 0 ? (int)std::min((long)16 * p.rt, rows) : 16 * p.rt;
+    p.tiles = T > 0 ? ceil_div(rows, per) : 0;
+    p.groups = T > 0 ? (long)B * p.tiles : n_tok * G / per + std::min((long)B, (long)n_tok);
+    const long blocks = ceil_div((long)width * c->page, 64);
+    const long want = ceil_div(512, p.groups * c->n_kv_heads);
+    p.n_split = (int)std::max(1l, std::min(std::min(want, 64l), (long)ceil_div(blocks, p.wk)));
+    return p;
+}
+
+template <int F, typename T, int D, int RT, int WK, int WR> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+{
+    const size_t lds = WK > 1 ? (size_t)WR * WK * p.lds_rows * (D + 2) * 4 : 0;
+    const dim3 grid((unsigned)p.groups, a.c.Hkv, p.n_split);
+    hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR>), grid, dim3(64 * WK * WR), lds, s, a);
+    UW_LAUNCH_CHECK();
+    return UW_OK;
+}
+
+template <int F, typename T, int D> int launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+{
+    int rc;
+    if (p.wr == 4) rc = launch_attention_as<F, T, D, 2, 1, 4>(a, p, s);
+    else if (p.rt == 1) rc = launch_attention_as<F, T, D, 1, 4, 1>(a, p, s);
+    else rc = launch_attention_as<F, T, D, 2, 4, 1>(a, p, s);
+    if (rc || p.n_split == 1) return rc;
+    hipLaunchKernelGGL((kv8_join_kernel<T, D>), dim3(ceil_div(a.ts.N * a.H, 4)), dim3(256), 0, s, a);
+    UW_LAUNCH_CHECK();
+    return UW_OK;
+}
+
 }  // namespace
 
 #define RUN(x)                   \
@@ -321,7 +661,9 @@ int uw_kv8_read(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, co
 
 int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_cache* cache, int n_heads, int B, int64_t n_tok, int T, int table_width)
 {
-    return 0;
+    if (check_cache("uw_kv8_attention_workspace_bytes", cache) || n_heads <= 0 || n_heads % cache->n_kv_heads || B <= 0 || n_tok <= 0) return 0;
+    const AttnPlan pl = plan_attention(cache, n_heads, B, n_tok, T, table_width);
+    return pl.n_split > 1 ? n_tok * n_heads * (int64_t)pl.n_split * (cache->head_dim + 4) * 4 : 0;
 }
 
 int uw_kv8_attention(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* q, const uw_kv8_tokens* o, float* lse, int n_heads,
@@ -334,12 +676,27 @@ int uw_kv8_attention(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* 
     RUN(check_table("uw_kv8_attention", table, table_width, kv_len));
     UW_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, "uw_kv8_attention: %d query heads over %d kv heads", n_heads, cache->n_kv_heads);
     if (q->n_tok == 0) return UW_OK;
-    const Kv8View c = view_of(cache, table, table_width);
-    const dim3 grid((unsigned)q->n_tok, n_heads);
-#define CALL(F, T) hipLaunchKernelGGL((kv8_attention_kernel<F, T>), grid, dim3(256), 0, (hipStream_t)stream, c, span_of(q), arg_of(q), arg_of(o), lse, n_heads, kv_len, causal, scale)
+    const AttnPlan pl = plan_attention(cache, n_heads, q->B, q->n_tok, q->tok_start ? 0 : q->T, table_width);
+    UW_REQUIRE(pl.n_split == 1 || (ws && ((uintptr_t)ws & 15) == 0), "uw_kv8_attention: workspace missing or misaligned");
+    UW_REQUIRE(pl.groups <= 0x7fffffff, "uw_kv8_attention: too many rows");
+    AttnArgs a;
+    a.c = view_of(cache, table, table_width);
+    a.ts = span_of(q);
+    a.q = arg_of(q);
+    a.o = arg_of(o);
+    a.lse = lse;
+    a.kv_len = kv_len;
+    a.part = (float*)ws;
+    a.H = n_heads;
+    a.G = n_heads / cache->n_kv_heads;
+    a.causal = causal;
+    a.n_split = pl.n_split;
+    a.tiles = pl.tiles;
+    a.lds_rows = pl.lds_rows;
+    a.scale2 = scale * LOG2E;
+#define CALL(F, T) RUN((cache->head_dim == 64 ? launch_attention<F, T, 64>(a, pl, (hipStream_t)stream) : launch_attention<F, T, 128>(a, pl, (hipStream_t)stream)))
     KV8_DISPATCH(cache->format, dtype, CALL);
 #undef CALL
-    UW_LAUNCH_CHECK();
     return UW_OK;
 }
 
