@@ -181,36 +181,52 @@ int uw_profile_span(uw_ctx* ctx, int kind, int64_t* launches_total, int64_t* lau
 typedef struct uw_kv8_cache {
     void *k, *v;
     float *k_scale, *v_scale;
-    int32_t n_pages, n_kv_heads, page, head_dim, format;
+    int32_t n_pages, n_kv_heads, page, head_dim, format, reserved;
 } uw_kv8_cache;
-typedef struct uw_kv8_tokens {      /* a [rows][heads][head_dim] array and how its rows belong to the sequences */
+typedef struct uw_kv8_seqs {        /* the sequences of a call and how the rows of its token arrays belong to them */
+    const int32_t *table, *len;     /* page table; [B] positions or lengths, see the calls */
+    const int32_t* tok_start;
+    int64_t n_tok;
+    int32_t table_width, B, T, dtype;
+} uw_kv8_seqs;
+typedef struct uw_kv8_tokens {      /* a [rows][heads][head_dim] array */
     void* data;
     int64_t seq_stride, tok_stride, head_stride;
-    int64_t n_tok;
-    const int32_t* tok_start;
-    int32_t B, T;
 } uw_kv8_tokens;
+typedef struct uw_kv8_store_args {
+    uw_kv8_cache cache;
+    uw_kv8_seqs seqs;
+    uw_kv8_tokens k, v;
+} uw_kv8_store_args;
+typedef struct uw_kv8_attention_args {
+    uw_kv8_cache cache;
+    uw_kv8_seqs seqs;
+    uw_kv8_tokens q, o;
+    float* lse;
+    void* ws;
+    int64_t ws_bytes;
+    int32_t n_heads, causal;
+    float scale;
+    int32_t reserved;
+} uw_kv8_attention_args;
 
-/* Appends keys and values: sequence b's tokens go to positions pos[b], pos[b] + 1, ... (pos i32 [B] = tokens already there).
+/* Appends keys and values: sequence b's tokens go to positions len[b], len[b] + 1, ... (len = tokens already there).
  * Per touched block, head and half: a block without earlier tokens takes its scale from the largest |x|; otherwise the scale
  * stays while the new values fit and grows by a power of two if not, the earlier tokens' codes being re-rounded.  A NaN or
  * infinity makes the scale of its block and head NaN until the block is begun again: whatever reads that block gives NaN.
- * A block of two sequences of one call must not be touched by both (shared prefixes end on a page boundary).  Codes behind the
- * last token are left as they are.  k->tok_start, B, T and n_tok hold for v too. */
-int uw_kv8_append(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, const uw_kv8_tokens* v, const int32_t* table,
-                  int table_width, const int32_t* pos, void* stream);
-/* Reads tokens back as values (code * scale, rounded once to dtype): positions first[b], first[b] + 1, ... into k and v. */
-int uw_kv8_read(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, const uw_kv8_tokens* v, const int32_t* table,
-                int table_width, const int32_t* first, void* stream);
+ * A block must not be touched by two sequences of one call (shared prefixes end on a page boundary).  Codes behind the last
+ * token are left as they are. */
+int uw_kv8_append(const uw_kv8_store_args* args, void* stream);
+/* Reads tokens back as values (code * scale, rounded once to dtype): positions len[b], len[b] + 1, ... into k and v. */
+int uw_kv8_read(const uw_kv8_store_args* args, void* stream);
 /* Attention of n_heads query heads (a multiple of n_kv_heads; query head h reads kv head h / (n_heads / n_kv_heads)) over the
- * first kv_len[b] cached tokens; with causal != 0 token t of the n tokens of a sequence sees keys 0 .. kv_len[b] - n + t (its
- * own key, appended before, is the last).  o: rows like q; lse (may be NULL) f32 [n_tok][n_heads]: log of the sum of exp(scores).
- * A row that sees no key gives 0 and lse = -inf.  scale multiplies q.k.  ws: uw_kv8_attention_workspace_bytes() bytes, 16-byte
- * aligned, not shared by calls that may run at the same time; NULL if that is 0. */
-int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_cache* cache, int n_heads, int B, int64_t n_tok, int T, int table_width);
-int uw_kv8_attention(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* q, const uw_kv8_tokens* o, float* lse, int n_heads,
-                     const int32_t* table, int table_width, const int32_t* kv_len, int causal, float scale, void* ws,
-                     void* stream);
+ * first len[b] cached tokens; with causal != 0 token t of the n tokens of a sequence sees keys 0 .. len[b] - n + t (its own
+ * key, appended before, is the last).  o: rows like q; lse (may be NULL) f32 [n_tok][n_heads]: log of the sum of exp(scores).
+ * A row that sees no key gives 0 and lse = -inf.  scale multiplies q.k.  ws: ws_bytes of scratch, at least what
+ * uw_kv8_attention_workspace_bytes() answers for the same arguments (it reads no device memory; -1: arguments refused),
+ * 16-byte aligned, not shared by calls that may run at the same time; NULL if that is 0. */
+int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_attention_args* args);
+int uw_kv8_attention(const uw_kv8_attention_args* args, void* stream);
 
 /* Verification of drafted tokens (speculative decoding): target [B][N+1][V] and draft [B][N][V] (NULL: the drafter is taken to
  * have been certain of its token) are logits, or probabilities if `probs`; rows at b * *_sB + i * *_sN, elements contiguous.
@@ -221,11 +237,24 @@ int uw_kv8_attention(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* 
  * is its row's arg-max (the lowest index of equal ones) and the next token is the arg-max; draft and uniforms are not read.
  * accepted i32 [B]; tokens i32 [B][N+1]: the accepted tokens, the next token, then -1.  The next token is -1 if its row holds
  * a NaN or has no mass (the decoder-run failure of core.py:948-956); a drafted id outside 0..V-1 is never accepted.
- * ws: uw_verify_draft_workspace_bytes() bytes, 16-byte aligned, not shared by calls that may run at the same time. */
-int64_t uw_verify_draft_workspace_bytes(int B, int N, int V);
-int uw_verify_draft(int dtype, const void* target, int64_t target_sB, int64_t target_sN, const void* draft, int64_t draft_sB,
-                    int64_t draft_sN, const int32_t* drafted, const int32_t* n_drafted, const float* uniforms, int B, int N, int V,
-                    float temperature, int probs, int32_t* accepted, int32_t* tokens, void* ws, void* stream);
+ * ws: ws_bytes of scratch, at least uw_verify_draft_workspace_bytes() (-1: arguments refused), 16-byte aligned, not shared by
+ * calls that may run at the same time. */
+typedef struct uw_verify_args {
+    const void* target;
+    int64_t target_sB, target_sN;
+    const void* draft;
+    int64_t draft_sB, draft_sN;
+    const int32_t *drafted, *n_drafted;
+    const float* uniforms;
+    int32_t *accepted, *tokens;
+    void* ws;
+    int64_t ws_bytes;
+    int32_t dtype, B, N, V;
+    float temperature;
+    int32_t probs;
+} uw_verify_args;
+int64_t uw_verify_draft_workspace_bytes(const uw_verify_args* args);
+int uw_verify_draft(const uw_verify_args* args, void* stream);
 
 #ifdef __cplusplus
 }

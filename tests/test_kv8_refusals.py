@@ -1,12 +1,10 @@
 """What the 8-bit cache's operators and the draft verification refuse, and how: no GPU is touched."""
-import ctypes as C
-
 import pytest
 import torch
 
 from whisper_amd import kv8
 from whisper_amd import lib as L
-from whisper_amd.speculative import verify_draft
+from whisper_amd.speculative import _ARGS, verify_draft
 
 
 def _cache(fmt="int8", pages=4, heads=2, page=16, dim=64):
@@ -40,7 +38,7 @@ def test_wrong_shapes_and_types_are_refused():
     table, pos = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
     x = torch.zeros(3, 5, 2, 64)
     for args, word in (((x[:2], x[:2], table, pos), "sequences"), ((x.half(), x.half(), table, pos), "float32 or bfloat16"),
-                       ((x[..., :32], x, table, pos), "float32 or bfloat16"), ((x, x[:, :4], table, pos), "alike"),
+                       ((x[..., :32], x[..., :32], table, pos), "float32 or bfloat16"), ((x, x[:, :4], table, pos), "alike"),
                        ((x[:, :, :1], x[:, :, :1], table, pos), "heads"), ((x, x, table.long(), pos), "page table"),
                        ((x, x, table[:, :0], pos), "page table"), ((x, x, table, pos[:2]), "pos"), ((x, x, table, pos.float()), "pos")):
         with pytest.raises(ValueError, match=word):
@@ -63,43 +61,50 @@ def test_wrong_shapes_and_types_are_refused():
 
 
 def test_library_refuses_before_any_gpu_call():
+    """The C entries check every size before they touch the GPU; the addresses here are none."""
     lib = L.load()
-    good = dict(k=64, v=64, k_scale=64, v_scale=64, n_pages=4, n_kv_heads=2, page=16, head_dim=64, format=L.UW_KV8_INT8)
-    tok = dict(data=64, seq_stride=128, tok_stride=128, head_stride=64, n_tok=3, tok_start=None, B=3, T=1)
+    good = dict(k=64, v=64, ks=64, vs=64, n_pages=4, heads=2, page=16, dim=64, fmt=L.UW_KV8_INT8, r=0, table=64, len=64, start=0,
+                n_tok=3, width=1, B=3, T=1, dtype=L.UW_DTYPE_BF16, x=64, sB=128, sT=128, sH=64, y=64, yB=128, yT=128, yH=64)
+    last = dict(lse=0, ws=0, ws_bytes=0, n_heads=2, causal=1, scale=0.125, r2=0)
 
-    def rc(cache=None, t=None, dtype=L.UW_DTYPE_BF16, heads=2, table=64, width=1, ln=64):
-        c, x = L.UwKv8Cache(**{**good, **(cache or {})}), L.UwKv8Tokens(**{**tok, **(t or {})})
-        out = []
-        out.append(lib.uw_kv8_append(C.byref(c), dtype, C.byref(x), C.byref(x), table, width, ln, None))
-        out.append(lib.uw_kv8_read(C.byref(c), dtype, C.byref(x), C.byref(x), table, width, ln, None))
-        out.append(lib.uw_kv8_attention(C.byref(c), dtype, C.byref(x), C.byref(x), None, heads, table, width, ln, 1, 0.125, None, None))
-        return out
+    def calls(**kw):
+        a = {**good, **{k: v for k, v in kw.items() if k in good}}
+        vals = list(a.values())
+        store = kv8._CACHE.pack(*vals[:10]) + kv8._STORE.pack(*vals[10:])
+        attend = kv8._CACHE.pack(*vals[:10]) + kv8._ATTEND.pack(*vals[10:], *{**last, **{k: v for k, v in kw.items() if k in last}}.values())
+        return (lambda: lib.uw_kv8_append(store, None), lambda: lib.uw_kv8_read(store, None), lambda: lib.uw_kv8_attention(attend, None),
+                lambda: lib.uw_kv8_attention_workspace_bytes(attend))
 
-    def refused(word, **kw):
-        assert all(r != 0 for r in rc(**kw)), (word, kw)
-        assert word.encode() in lib.uw_last_error(), lib.uw_last_error()
+    def refused(word, which=range(4), **kw):
+        for i in which:
+            rc = calls(**kw)[i]()
+            assert (rc == -1) if i == 3 else rc > 0, (word, i, rc)
+            assert word.encode() in lib.uw_last_error(), (i, lib.uw_last_error())
 
-    refused("null cache", cache={"k": None})
-    refused("format", cache={"format": 2})
-    refused("tokens", cache={"page": 48})
-    refused("head_dim", cache={"head_dim": 96})
-    refused("pages", cache={"n_pages": 0})
-    refused("aligned", cache={"v": 72})
+    refused("null cache", k=0)
+    refused("format", fmt=2)
+    refused("tokens", page=48)
+    refused("head_dim", dim=96)
+    refused("pages", n_pages=0)
+    refused("aligned", v=72)
     refused("dtype", dtype=7)
-    refused("sequences", t={"B": 0})
-    refused("null data", t={"data": None})
-    refused("rows", t={"n_tok": 4})
-    refused("multiples", t={"tok_stride": 130})
-    refused("null page table", table=None)
+    refused("sequences", B=0)
+    refused("null data", x=0)
+    refused("rows are not", n_tok=4)
+    refused("too many rows", n_tok=1 << 40, start=64)
+    refused("multiples", sT=130)
+    refused("multiples", y=72)
+    refused("null page table", table=0)
     refused("null page table", width=0)
-    c, x = L.UwKv8Cache(**good), L.UwKv8Tokens(**tok)
-    assert lib.uw_kv8_attention(C.byref(c), 1, C.byref(x), C.byref(x), None, 3, 64, 1, 64, 1, 0.125, None, None) != 0
-    assert b"query heads" in lib.uw_last_error()
-    y = L.UwKv8Tokens(**{**tok, "B": 1, "T": 3})
-    assert lib.uw_kv8_append(C.byref(c), 1, C.byref(x), C.byref(y), 64, 1, 64, None) != 0 and b"same tokens" in lib.uw_last_error()
-    # nothing to do is no error
-    z = L.UwKv8Tokens(**{**tok, "T": 0, "n_tok": 0})
-    assert lib.uw_kv8_append(C.byref(c), 1, C.byref(z), C.byref(z), 64, 1, 64, None) == 0
+    refused("columns", width=1 << 24)
+    refused("query heads", (2, 3), n_heads=3)
+    refused("workspace", (2,), width=4096)                    # long enough to be split over workgroups, and no workspace
+    assert calls(width=4096)[3]() > 0
+    refused("workspace", (2,), width=4096, ws=64, ws_bytes=16)
+    for call in calls(T=0, n_tok=0)[:3]:                      # nothing to do is no error
+        assert call() == 0
+    for fn in (lib.uw_kv8_append, lib.uw_kv8_read, lib.uw_kv8_attention):
+        assert fn(None, None) > 0 and b"null arguments" in lib.uw_last_error()
 
 
 def test_verify_draft_refuses():
@@ -115,7 +120,13 @@ def test_verify_draft_refuses():
     with pytest.raises(L.UwError, match="GPU"):
         verify_draft(t, d, u)
     lib = L.load()
-    assert lib.uw_verify_draft(0, None, 0, 0, None, 0, 0, None, None, None, 1, 1, 1, 1.0, 0, None, None, None, None) != 0
-    assert lib.uw_verify_draft(3, 64, 0, 0, None, 0, 0, 64, None, 64, 1, 1, 1, 1.0, 0, 64, 64, 64, None) != 0
-    assert lib.uw_verify_draft(0, 66, 0, 0, None, 0, 0, 64, None, 64, 1, 1, 1, 1.0, 0, 64, 64, 64, None) != 0
-    assert b"misaligned" in lib.uw_last_error()
+    good = dict(target=64, sB=20, sN=10, draft=0, dB=0, dN=0, drafted=64, n_drafted=0, uniforms=64, accepted=64, tokens=64, ws=0, ws_bytes=0,
+                dtype=0, B=1, N=1, V=10, temperature=1.0, probs=0)
+    for kw, word in ((dict(target=0), "null"), (dict(tokens=0), "null"), (dict(drafted=0), "null"), (dict(dtype=3), "dtype"), (dict(V=0), "V 0"),
+                     (dict(N=-1), "N -1"), (dict(B=0), "B 0"), (dict(uniforms=0), "uniforms"), (dict(temperature=-0.5), "temperature"),
+                     (dict(temperature=float("nan")), "temperature"), (dict(temperature=0.5, probs=1), "temperature"),
+                     (dict(target=66), "misaligned"), (dict(draft=65), "misaligned")):
+        args = _ARGS.pack(*{**good, **kw}.values())
+        assert lib.uw_verify_draft(args, None) > 0 and word.encode() in lib.uw_last_error(), (kw, lib.uw_last_error())
+        assert lib.uw_verify_draft_workspace_bytes(args) == -1
+    assert lib.uw_verify_draft(None, None) > 0

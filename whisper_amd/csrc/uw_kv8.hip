@@ -145,9 +145,10 @@ struct AttnArgs {
     const int32_t* kv_len;
     float* part;         // [rows][H][n_split][D + 4] partial results (output, maximum, sum) when n_split > 1
     int H, G, causal, n_split;
-    int tiles;           // workgroups per sequence (uniform)
+    int tiles, groups;   // workgroups per sequence (uniform), and of all sequences
     int lds_rows;        // rows of a tile that can be in use
-    float scale2;        // scale * log2(e)
+    float scale2;        // |scale| * log2(e)
+    unsigned neg;        // sign bit of scale, moved to the queries
 };
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -199,6 +200,23 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int n)
     return make_uint4(v.x & m(n), v.y & m(n - 4), v.z & m(n - 8), v.w & m(n - 12));
 }
 
+// a 16-byte piece of the cache; ONCE: no other workgroup will want it, so it need not stay in L2
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+template <bool ONCE> __device__ __forceinline__ uint4 ld_codes(const void* p)
+{
+    const u32x4 v = ONCE ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// largest of the four lanes that hold a row (lane & 15 alike), without a trip through LDS; a NaN loses
+__device__ __forceinline__ float across_groups_max(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 // four channels of a finished row (or of a split's part of it)
 template <typename T, int D>
 __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first, int kvh, int row, int d, int split, float M, float L, f32x4 acc)
@@ -220,7 +238,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
 
 // WK waves share the keys of a row tile (their results are joined in LDS), WR row tiles per workgroup
 template <int F, typename T, int D, int RT, int WK, int WR>
-__global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
+__global__ __launch_bounds__(64 * WK * WR, (RT * D <= 64 && sizeof(T) == 2) ? 4 : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -229,15 +247,17 @@ __global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
     const Kv8View& c = p.c;
 
     // which sequence, kv head, rows
+    // (heads run fastest: the workgroups of a head land on one XCD when their number is a multiple of 8, and share its L2)
     int b, tile;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    const int kvh = blockIdx.x % c.Hkv, rest = blockIdx.x / c.Hkv, split = rest / p.groups, group = rest % p.groups;
     if (p.ts.tok_start) {
-        if (!locate(blockIdx.x, p.ts.B, [&](int i) { return (int)(((long)p.ts.count(i) * p.G + ROWS * WR - 1) / (ROWS * WR)); }, b, tile)) return;
+        if (!locate(group, p.ts.B, [&](int i) { return (int)(((long)p.ts.count(i) * p.G + ROWS * WR - 1) / (ROWS * WR)); }, b, tile)) return;
     } else {
-        b = blockIdx.x / p.tiles;
-        tile = blockIdx.x % p.tiles;
+        b = group / p.tiles;
+        tile = group % p.tiles;
     }
     const int n = p.ts.count(b), n_rows = n * p.G;
+    if (p.causal) tile = (n_rows + ROWS * WR - 1) / (ROWS * WR) - 1 - tile;      // rows that see most first
     const int row0 = (tile * WR + wr) * ROWS;
     const int len = max(0, p.kv_len[b]);
     const long t_first = p.ts.first(b);
@@ -264,11 +284,16 @@ __global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
                 if constexpr (NP == 1) {
                     uint4 w = make_uint4(0, 0, 0, 0);
                     if (row < n_rows) w = *(const uint4*)((const T*)p.q.data + at + hf * 64 + s * 8);
+                    const unsigned flip = p.neg | p.neg >> 16;
+                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
                     qf[i][hf][s][0] = __builtin_bit_cast(bf16x8, w);
                 } else {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = row < n_rows ? to_f32<T>(((const T*)p.q.data)[at + hf * 64 + s * 8 + e]) : 0.f;
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = row < n_rows ? to_f32<T>(((const T*)p.q.data)[at + hf * 64 + s * 8 + e]) : 0.f;
+                        x[e] = __uint_as_float(__float_as_uint(x[e]) ^ p.neg);
+                    }
                     planes<NP>(x, qf[i][hf][s]);
                 }
             }
@@ -289,30 +314,40 @@ __global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
     const int per = (blocks + p.n_split - 1) / p.n_split;
     const int blk1 = min(blocks, (split + 1) * per);
     const long page_bytes = (long)c.P * D;
-    const bool small = c.P < 64;
-    const int k_group = rr >> 2, k_in = rr & 3;     // 16-key group and place in it of this lane's K rows
-    for (int blk = split * per + wk; blk < blk1; blk += WK) {
-        const int j0 = blk << 6, jk = j0 + 16 * k_group, jv = j0 + 16 * g4;
-        int pk, pv;
-        if (small) {
-            pk = kv8_page(c, b, jk >> c.log2P);
-            pv = kv8_page(c, b, jv >> c.log2P);
-        } else {
-            pk = pv = kv8_page(c, b, j0 >> c.log2P);
-        }
-        const uint8_t* kp = c.k + ((long)max(pk, 0) * c.Hkv + kvh) * page_bytes + ((jk & (c.P - 1)) + k_in) * D + g4 * 16;
-        const uint8_t* vp = c.v + ((long)max(pv, 0) * c.Hkv + kvh) * page_bytes + (long)rr * c.P + (jv & (c.P - 1));
-        uint4 kf[4][HALF], vf[D / 16];
+    const int k_group = 16 * (rr >> 2), k_in = rr & 3;     // 16-key group and place in it of this lane's K rows
+    uint4 kf[4][HALF], vf[D / 16];
+    float ks, vs;
+    int pk, pv;                                            // pages of this lane's K rows and of its 16 keys of V (alike from 64 tokens a page)
+    auto pages_of = [&](int blk) {
+        pv = kv8_page(c, b, ((blk << 6) + 16 * g4) >> c.log2P);
+        pk = c.P < 64 ? kv8_page(c, b, ((blk << 6) + k_group) >> c.log2P) : pv;
+    };
+    auto load_k = [&](int blk) {
+        const uint8_t* kp = c.k + ((long)max(pk, 0) * c.Hkv + kvh) * page_bytes + ((((blk << 6) + k_group) & (c.P - 1)) + k_in) * D + g4 * 16;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = *(const uint4*)(kp + t * 4 * D + hf * 64);
+            for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = ld_codes<(WR == 1)>(kp + t * 4 * D + hf * 64);
+        ks = c.ks[(long)max(pv, 0) * c.Hkv + kvh];
+    };
+    auto load_v = [&](int blk) {
+        const uint8_t* vp = c.v + ((long)max(pv, 0) * c.Hkv + kvh) * page_bytes + rr * c.P + (((blk << 6) + 16 * g4) & (c.P - 1));
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) vf[d] = *(const uint4*)(vp + (long)d * 16 * c.P);
+        for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(WR == 1)>(vp + d * 16 * c.P);
+        vs = c.vs[(long)max(pv, 0) * c.Hkv + kvh];
+    };
+    int blk = split * per + wk;
+    if (blk < blk1) {
+        pages_of(blk);
+        load_k(blk);
+        load_v(blk);
+    }
+    for (; blk < blk1; blk += WK) {
+        const int j0 = blk << 6, jv = j0 + 16 * g4;
+        const bool mask = lim_min - j0 < 64, more = blk + WK < blk1;
         const float nan = __uint_as_float(0x7fc00000u);
-        const float ks = pv < 0 ? nan : c.ks[(long)pv * c.Hkv + kvh] * p.scale2;
-        const float vs = pv < 0 ? nan : c.vs[(long)pv * c.Hkv + kvh];
-        const bool mask = lim_min - j0 < 64;
+        const float kscale = pv < 0 ? nan : ks * p.scale2;
+        if (more) pages_of(blk + WK);
 
         f32x4 st[RT][4];
 #pragma unroll
@@ -332,16 +367,16 @@ __global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
                         st[i][t] = mfma(a1, qf[i][hf][1][pl], st[i][t]);
                     }
             }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_k(blk + WK);          // in flight under the softmax and P.V
+        __builtin_amdgcn_sched_barrier(0);
+
+        // a block of zeros (scale 0) has codes of zero: any scale does.  The V scale rides in the exponent: p' = p * vs costs nothing per
+        // element, the sum is divided by it once per block (the rounding of log2(vs) adds |log2 vs| 2^-24 to an element)
+        const float vsc = vs == 0.f ? 1.f : vs, lv = __builtin_amdgcn_logf(vsc), iv = __builtin_amdgcn_rcpf(vsc);
         bf16x8 pf[RT][2][NP];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    st[i][t][e] *= ks;
-                }
             const int left = lim[i] - jv;          // keys of this lane's 16 that the row sees
             if (mask) {
 #pragma unroll
@@ -350,35 +385,35 @@ __global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
                     for (int e = 0; e < 4; ++e)
                         if (4 * t + e >= left) st[i][t][e] = -INFINITY;
             }
+            float mx = fmaxf(st[i][0][0], st[i][0][1]);
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[i][t][e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            for (int k = 2; k < 16; k += 2) mx = fmaxf(fmaxf(mx, st[i][k >> 2][k & 3]), st[i][k >> 2][(k & 3) + 1]);
+            mx *= kscale;
+            if (mask && left <= 0) mx = -INFINITY;      // nothing of these 16 keys is seen, and the scale may be any leftover
+            mx = across_groups_max(mx);
             const float mn = fmaxf(m[i], mx);
             const float base = mn == -INFINITY ? 0.f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
             if (__any(mn != m[i])) {
+                const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
                 l[i] *= alpha;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) o[i][d] *= alpha;
+                m[i] = mn;
             }
-            m[i] = mn;
+            const float nb = lv - base;
             float x[16];
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float pr = __builtin_amdgcn_exp2f(st[i][t][e] - base);
-                    l[i] += pr;
-                    x[4 * t + e] = pr * vs;
-                }
+            for (int k = 0; k < 16; ++k) x[k] = __builtin_amdgcn_exp2f(fmaf(st[i][k >> 2][k & 3], kscale, nb));
             if (mask) {                            // a scale behind the end may be NaN
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
                     if (k >= left) x[k] = 0.f;
             }
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sum += x[k];
+            // (a poisoned scale of a block that is seen shows in the sum)
+            if (!mask || left > 0) l[i] = fmaf(sum, iv, l[i]);
             planes<NP>(x, pf[i][0]);
             planes<NP>(x + 8, pf[i][1]);
         }
@@ -398,6 +433,9 @@ __global__ __launch_bounds__(64 * WK * WR) void kv8_attention_kernel(AttnArgs p)
                     o[i][d] = mfma(a1, pf[i][1][pl], o[i][d]);
                 }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_v(blk + WK);
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -481,6 +519,12 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p)
 }
 
 // ---- host side --------------------------------------------------------------------------------------
+#define RUN(x)                   \
+    do {                         \
+        const int rc__ = (x);    \
+        if (rc__) return rc__;   \
+    } while (0)
+
 int log2_page(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : page == 256 ? 8 : -1; }
 
 int check_cache(const char* fn, const uw_kv8_cache* c)
@@ -495,35 +539,28 @@ int check_cache(const char* fn, const uw_kv8_cache* c)
     return UW_OK;
 }
 
-int check_tokens(const char* fn, const char* what, const uw_kv8_tokens* t, int dtype)
+int check_seqs(const char* fn, const uw_kv8_seqs* t)
 {
-    UW_REQUIRE(dtype == UW_DTYPE_F32 || dtype == UW_DTYPE_BF16, "%s: dtype must be f32 or bf16", fn);
-    const int unit = dtype == UW_DTYPE_F32 ? 4 : 8;      // elements in 16 bytes
-    UW_REQUIRE(t && t->B > 0 && t->n_tok >= 0, "%s: %s: %d sequences", fn, what, t ? t->B : 0);
-    UW_REQUIRE(t->n_tok == 0 || t->data, "%s: %s: null data", fn, what);
-    UW_REQUIRE(t->tok_start || (t->T >= 0 && t->n_tok == (int64_t)t->B * t->T), "%s: %s: %lld rows are not %d x %d", fn, what,
+    UW_REQUIRE(t->dtype == UW_DTYPE_F32 || t->dtype == UW_DTYPE_BF16, "%s: dtype must be f32 or bf16", fn);
+    UW_REQUIRE(t->B > 0 && t->n_tok >= 0, "%s: %d sequences, %lld rows", fn, t->B, (long long)t->n_tok);
+    UW_REQUIRE(t->tok_start || (t->T >= 0 && t->n_tok == (int64_t)t->B * t->T), "%s: %lld rows are not %d x %d", fn,
                (long long)t->n_tok, t->B, t->T);
-    UW_REQUIRE(t->n_tok <= 0x7fffffff, "%s: %s: too many rows", fn, what);
+    UW_REQUIRE(t->n_tok <= 0x7fffffff, "%s: too many rows", fn);
+    UW_REQUIRE(t->table && t->len && t->table_width > 0, "%s: null page table or lengths, or no columns", fn);
+    UW_REQUIRE(t->table_width <= (1 << 23), "%s: %d table columns", fn, t->table_width);
+    return UW_OK;
+}
+
+int check_tokens(const char* fn, const char* what, const uw_kv8_tokens* t, const uw_kv8_seqs* q)
+{
+    const int unit = q->dtype == UW_DTYPE_F32 ? 4 : 8;      // elements in 16 bytes
+    UW_REQUIRE(q->n_tok == 0 || t->data, "%s: %s: null data", fn, what);
     UW_REQUIRE(((uintptr_t)t->data & 15) == 0 && t->seq_stride % unit == 0 && t->tok_stride % unit == 0 && t->head_stride % unit == 0,
                "%s: %s: base and strides must be multiples of 16 bytes", fn, what);
     return UW_OK;
 }
 
-int check_table(const char* fn, const int32_t* table, int width, const int32_t* len)
-{
-    UW_REQUIRE(table && len && width > 0, "%s: null page table or lengths, or no columns", fn);
-    UW_REQUIRE(width <= (1 << 23), "%s: %d table columns", fn, width);
-    return UW_OK;
-}
-
-int check_pair(const char* fn, const uw_kv8_tokens* k, const uw_kv8_tokens* v)
-{
-    UW_REQUIRE(k->tok_start == v->tok_start && k->B == v->B && k->n_tok == v->n_tok && (k->tok_start || k->T == v->T),
-               "%s: k and v must hold the same tokens", fn);
-    return UW_OK;
-}
-
-Kv8View view_of(const uw_kv8_cache* c, const int32_t* table, int width)
+Kv8View view_of(const uw_kv8_cache* c, const uw_kv8_seqs* q)
 {
     Kv8View v;
     v.k = (uint8_t*)c->k;
@@ -535,16 +572,16 @@ Kv8View view_of(const uw_kv8_cache* c, const int32_t* table, int width)
     v.P = c->page;
     v.log2P = log2_page(c->page);
     v.D = c->head_dim;
-    v.table = table;
-    v.width = width;
+    v.table = q->table;
+    v.width = q->table_width;
     return v;
 }
 
 TokArg arg_of(const uw_kv8_tokens* t) { return TokArg{t->data, (long)t->seq_stride, (long)t->tok_stride, (long)t->head_stride}; }
-TokSpan span_of(const uw_kv8_tokens* t) { return TokSpan{t->tok_start, t->B, t->T, (long)t->n_tok}; }
+TokSpan span_of(const uw_kv8_seqs* t) { return TokSpan{t->tok_start, t->B, t->T, (long)t->n_tok}; }
 
 // upper bound of the blocks a call touches, known without reading the lengths: n tokens touch at most (n - 1) / P + 2
-long touched_bound(const uw_kv8_tokens* t, int P)
+long touched_bound(const uw_kv8_seqs* t, int P)
 {
     if (t->tok_start) return t->n_tok / P + 2l * std::min((long)t->B, (long)t->n_tok);
     return (long)t->B * ((t->T + P - 2) / P + 1);
@@ -559,18 +596,42 @@ long touched_bound(const uw_kv8_tokens* t, int P)
         }                                                                                   \
     } while (0)
 
+int check_store(const char* fn, const uw_kv8_store_args* a)
+{
+    UW_REQUIRE(a, "%s: null arguments", fn);
+    RUN(check_cache(fn, &a->cache));
+    RUN(check_seqs(fn, &a->seqs));
+    RUN(check_tokens(fn, "k", &a->k, &a->seqs));
+    RUN(check_tokens(fn, "v", &a->v, &a->seqs));
+    UW_REQUIRE(touched_bound(&a->seqs, a->cache.page) < (1 << 24), "%s: too many rows", fn);
+    return UW_OK;
+}
+
+int check_attention(const char* fn, const uw_kv8_attention_args* a)
+{
+    UW_REQUIRE(a, "%s: null arguments", fn);
+    RUN(check_cache(fn, &a->cache));
+    RUN(check_seqs(fn, &a->seqs));
+    RUN(check_tokens(fn, "q", &a->q, &a->seqs));
+    RUN(check_tokens(fn, "o", &a->o, &a->seqs));
+    UW_REQUIRE(a->n_heads > 0 && a->n_heads % a->cache.n_kv_heads == 0, "%s: %d query heads over %d kv heads", fn, a->n_heads, a->cache.n_kv_heads);
+    return UW_OK;
+}
+
 struct AttnPlan {
     int rt, wk, wr;      // row tiles of 16 per wave, waves sharing keys, waves side by side on rows
     int n_split, tiles, lds_rows;
-    long groups;         // grid.x
+    long groups, ws_bytes;
 };
 
 // How a call is cut.  Few rows per sequence: the waves of a workgroup share the keys, and the keys are cut over workgroups until
 // the chip is full.  Many rows: the waves take rows of their own.
-AttnPlan plan_attention(const uw_kv8_cache* c, int n_heads, int B, int64_t n_tok, int T, int width)
+AttnPlan plan_attention(const uw_kv8_attention_args* a)
 {
     AttnPlan p;
-    const int G = n_heads / c->n_kv_heads;
+    const uw_kv8_cache* c = &a->cache;
+    const int G = a->n_heads / c->n_kv_heads, B = a->seqs.B, T = a->seqs.tok_start ? 0 : a->seqs.T, width = a->seqs.table_width;
+    const int64_t n_tok = a->seqs.n_tok;
     const long rows = T > 0 ? (long)T * G : (long)ceil_div(n_tok, B) * G;     // per sequence; packed: on average
     const int max_rt = 2;
     if (rows <= 16 * max_rt * 2) {
@@ -589,13 +650,14 @@ AttnPlan plan_attention(const uw_kv8_cache* c, int n_heads, int B, int64_t n_tok
     const long blocks = ceil_div((long)width * c->page, 64);
     const long want = ceil_div(512, p.groups * c->n_kv_heads);
     p.n_split = (int)std::max(1l, std::min(std::min(want, 64l), (long)ceil_div(blocks, p.wk)));
+    p.ws_bytes = p.n_split > 1 ? n_tok * a->n_heads * (int64_t)p.n_split * (c->head_dim + 4) * 4 : 0;
     return p;
 }
 
 template <int F, typename T, int D, int RT, int WK, int WR> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
 {
     const size_t lds = WK > 1 ? (size_t)WR * WK * p.lds_rows * (D + 2) * 4 : 0;
-    const dim3 grid((unsigned)p.groups, a.c.Hkv, p.n_split);
+    const dim3 grid((unsigned)(p.groups * a.c.Hkv * p.n_split));
     hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR>), grid, dim3(64 * WK * WR), lds, s, a);
     UW_LAUNCH_CHECK();
     return UW_OK;
@@ -615,87 +677,68 @@ template <int F, typename T, int D> int launch_attention(const AttnArgs& a, cons
 
 }  // namespace
 
-#define RUN(x)                   \
-    do {                         \
-        const int rc__ = (x);    \
-        if (rc__) return rc__;   \
-    } while (0)
-
 extern "C" {
 
-int uw_kv8_append(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, const uw_kv8_tokens* v, const int32_t* table,
-                  int table_width, const int32_t* pos, void* stream)
+int uw_kv8_append(const uw_kv8_store_args* a, void* stream)
 {
-    RUN(check_cache("uw_kv8_append", cache));
-    RUN(check_tokens("uw_kv8_append", "k", k, dtype));
-    RUN(check_tokens("uw_kv8_append", "v", v, dtype));
-    RUN(check_pair("uw_kv8_append", k, v));
-    RUN(check_table("uw_kv8_append", table, table_width, pos));
-    if (k->n_tok == 0) return UW_OK;
-    const Kv8View c = view_of(cache, table, table_width);
-    const dim3 grid((unsigned)touched_bound(k, c.P), c.Hkv, 2);
-#define CALL(F, T) hipLaunchKernelGGL((kv8_append_kernel<F, T>), grid, dim3(256), 0, (hipStream_t)stream, c, span_of(k), arg_of(k), arg_of(v), pos)
-    KV8_DISPATCH(cache->format, dtype, CALL);
+    RUN(check_store("uw_kv8_append", a));
+    if (a->seqs.n_tok == 0) return UW_OK;
+    const Kv8View c = view_of(&a->cache, &a->seqs);
+    const dim3 grid((unsigned)touched_bound(&a->seqs, c.P), c.Hkv, 2);
+#define CALL(F, T) hipLaunchKernelGGL((kv8_append_kernel<F, T>), grid, dim3(256), 0, (hipStream_t)stream, c, span_of(&a->seqs), arg_of(&a->k), arg_of(&a->v), a->seqs.len)
+    KV8_DISPATCH(a->cache.format, a->seqs.dtype, CALL);
 #undef CALL
     UW_LAUNCH_CHECK();
     return UW_OK;
 }
 
-int uw_kv8_read(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* k, const uw_kv8_tokens* v, const int32_t* table,
-                int table_width, const int32_t* first, void* stream)
+int uw_kv8_read(const uw_kv8_store_args* a, void* stream)
 {
-    RUN(check_cache("uw_kv8_read", cache));
-    RUN(check_tokens("uw_kv8_read", "k", k, dtype));
-    RUN(check_tokens("uw_kv8_read", "v", v, dtype));
-    RUN(check_pair("uw_kv8_read", k, v));
-    RUN(check_table("uw_kv8_read", table, table_width, first));
-    if (k->n_tok == 0) return UW_OK;
-    const Kv8View c = view_of(cache, table, table_width);
-    const dim3 grid((unsigned)touched_bound(k, c.P), c.Hkv, 2);
-#define CALL(F, T) hipLaunchKernelGGL((kv8_read_kernel<F, T>), grid, dim3(256), 0, (hipStream_t)stream, c, span_of(k), arg_of(k), arg_of(v), first)
-    KV8_DISPATCH(cache->format, dtype, CALL);
+    RUN(check_store("uw_kv8_read", a));
+    if (a->seqs.n_tok == 0) return UW_OK;
+    const Kv8View c = view_of(&a->cache, &a->seqs);
+    const dim3 grid((unsigned)touched_bound(&a->seqs, c.P), c.Hkv, 2);
+#define CALL(F, T) hipLaunchKernelGGL((kv8_read_kernel<F, T>), grid, dim3(256), 0, (hipStream_t)stream, c, span_of(&a->seqs), arg_of(&a->k), arg_of(&a->v), a->seqs.len)
+    KV8_DISPATCH(a->cache.format, a->seqs.dtype, CALL);
 #undef CALL
     UW_LAUNCH_CHECK();
     return UW_OK;
 }
 
-int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_cache* cache, int n_heads, int B, int64_t n_tok, int T, int table_width)
+int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_attention_args* a)
 {
-    if (check_cache("uw_kv8_attention_workspace_bytes", cache) || n_heads <= 0 || n_heads % cache->n_kv_heads || B <= 0 || n_tok <= 0) return 0;
-    const AttnPlan pl = plan_attention(cache, n_heads, B, n_tok, T, table_width);
-    return pl.n_split > 1 ? n_tok * n_heads * (int64_t)pl.n_split * (cache->head_dim + 4) * 4 : 0;
+    if (check_attention("uw_kv8_attention_workspace_bytes", a)) return -1;
+    return a->seqs.n_tok ? plan_attention(a).ws_bytes : 0;
 }
 
-int uw_kv8_attention(const uw_kv8_cache* cache, int dtype, const uw_kv8_tokens* q, const uw_kv8_tokens* o, float* lse, int n_heads,
-                     const int32_t* table, int table_width, const int32_t* kv_len, int causal, float scale, void* ws, void* stream)
+int uw_kv8_attention(const uw_kv8_attention_args* a, void* stream)
 {
-    RUN(check_cache("uw_kv8_attention", cache));
-    RUN(check_tokens("uw_kv8_attention", "q", q, dtype));
-    RUN(check_tokens("uw_kv8_attention", "o", o, dtype));
-    RUN(check_pair("uw_kv8_attention", q, o));
-    RUN(check_table("uw_kv8_attention", table, table_width, kv_len));
-    UW_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, "uw_kv8_attention: %d query heads over %d kv heads", n_heads, cache->n_kv_heads);
-    if (q->n_tok == 0) return UW_OK;
-    const AttnPlan pl = plan_attention(cache, n_heads, q->B, q->n_tok, q->tok_start ? 0 : q->T, table_width);
-    UW_REQUIRE(pl.n_split == 1 || (ws && ((uintptr_t)ws & 15) == 0), "uw_kv8_attention: workspace missing or misaligned");
-    UW_REQUIRE(pl.groups <= 0x7fffffff, "uw_kv8_attention: too many rows");
-    AttnArgs a;
-    a.c = view_of(cache, table, table_width);
-    a.ts = span_of(q);
-    a.q = arg_of(q);
-    a.o = arg_of(o);
-    a.lse = lse;
-    a.kv_len = kv_len;
-    a.part = (float*)ws;
-    a.H = n_heads;
-    a.G = n_heads / cache->n_kv_heads;
-    a.causal = causal;
-    a.n_split = pl.n_split;
-    a.tiles = pl.tiles;
-    a.lds_rows = pl.lds_rows;
-    a.scale2 = scale * LOG2E;
-#define CALL(F, T) RUN((cache->head_dim == 64 ? launch_attention<F, T, 64>(a, pl, (hipStream_t)stream) : launch_attention<F, T, 128>(a, pl, (hipStream_t)stream)))
-    KV8_DISPATCH(cache->format, dtype, CALL);
+    RUN(check_attention("uw_kv8_attention", a));
+    const uw_kv8_seqs& q = a->seqs;
+    if (q.n_tok == 0) return UW_OK;
+    const AttnPlan pl = plan_attention(a);
+    UW_REQUIRE(pl.ws_bytes == 0 || (a->ws && ((uintptr_t)a->ws & 15) == 0 && a->ws_bytes >= pl.ws_bytes),
+               "uw_kv8_attention: workspace missing, misaligned or smaller than %lld bytes", (long long)pl.ws_bytes);
+    UW_REQUIRE(pl.groups * a->cache.n_kv_heads * pl.n_split < (1 << 24) && q.n_tok * a->n_heads <= 0x7fffffff, "uw_kv8_attention: too many rows");
+    AttnArgs x;
+    x.c = view_of(&a->cache, &q);
+    x.ts = span_of(&q);
+    x.q = arg_of(&a->q);
+    x.o = arg_of(&a->o);
+    x.lse = a->lse;
+    x.kv_len = q.len;
+    x.part = (float*)a->ws;
+    x.H = a->n_heads;
+    x.G = a->n_heads / a->cache.n_kv_heads;
+    x.causal = a->causal;
+    x.n_split = pl.n_split;
+    x.tiles = pl.tiles;
+    x.groups = (int)pl.groups;
+    x.lds_rows = pl.lds_rows;
+    x.scale2 = fabsf(a->scale) * LOG2E;
+    x.neg = a->scale < 0.f ? 0x80000000u : 0u;
+#define CALL(F, T) RUN((a->cache.head_dim == 64 ? launch_attention<F, T, 64>(x, pl, (hipStream_t)stream) : launch_attention<F, T, 128>(x, pl, (hipStream_t)stream)))
+    KV8_DISPATCH(a->cache.format, q.dtype, CALL);
 #undef CALL
     return UW_OK;
 }

@@ -178,28 +178,35 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyParams p)
     for (int i = tid; i <= p.N; i += 256) p.tokens[(long)b * (p.N + 1) + i] = i < acc ? d[i] : i == acc ? next : -1;
 }
 
+int check_verify(const uw_verify_args* a)
+{
+    UW_REQUIRE(a, "uw_verify_draft: null arguments");
+    UW_REQUIRE(a->dtype == UW_DTYPE_F32 || a->dtype == UW_DTYPE_BF16, "uw_verify_draft: dtype must be f32 or bf16");
+    UW_REQUIRE(a->B > 0 && a->N >= 0 && a->V > 0, "uw_verify_draft: B %d, N %d, V %d", a->B, a->N, a->V);
+    UW_REQUIRE(a->target && a->accepted && a->tokens && (a->drafted || a->N == 0), "uw_verify_draft: null argument");
+    UW_REQUIRE(a->temperature >= 0.f && a->temperature < INFINITY, "uw_verify_draft: temperature must be finite and not negative");
+    UW_REQUIRE(a->uniforms || a->temperature == 0.f, "uw_verify_draft: uniforms missing");
+    UW_REQUIRE(!a->probs || a->temperature == 1.f || a->temperature == 0.f, "uw_verify_draft: probabilities take no temperature");
+    UW_REQUIRE((((uintptr_t)a->target | (uintptr_t)a->draft) & (a->dtype == UW_DTYPE_F32 ? 3 : 1)) == 0, "uw_verify_draft: misaligned rows");
+    return UW_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
-int64_t uw_verify_draft_workspace_bytes(int B, int N, int V) { return 0; }
+int64_t uw_verify_draft_workspace_bytes(const uw_verify_args* a) { return check_verify(a) ? -1 : 0; }
 
-int uw_verify_draft(int dtype, const void* target, int64_t target_sB, int64_t target_sN, const void* draft, int64_t draft_sB,
-                    int64_t draft_sN, const int32_t* drafted, const int32_t* n_drafted, const float* uniforms, int B, int N, int V,
-                    float temperature, int probs, int32_t* accepted, int32_t* tokens, void* ws, void* stream)
+int uw_verify_draft(const uw_verify_args* a, void* stream)
 {
-    UW_REQUIRE(dtype == UW_DTYPE_F32 || dtype == UW_DTYPE_BF16, "uw_verify_draft: dtype must be f32 or bf16");
-    UW_REQUIRE(B > 0 && N >= 0 && V > 0, "uw_verify_draft: B %d, N %d, V %d", B, N, V);
-    UW_REQUIRE(target && accepted && tokens && (drafted || N == 0), "uw_verify_draft: null argument");
-    UW_REQUIRE(temperature >= 0.f && temperature < INFINITY, "uw_verify_draft: temperature must be finite and not negative");
-    UW_REQUIRE(uniforms || temperature == 0.f, "uw_verify_draft: uniforms missing");
-    UW_REQUIRE(!probs || temperature == 1.f || temperature == 0.f, "uw_verify_draft: probabilities take no temperature");
-    const int es = dtype == UW_DTYPE_F32 ? 4 : 2;
-    UW_REQUIRE((((uintptr_t)target | (uintptr_t)draft) & (es - 1)) == 0, "uw_verify_draft: misaligned rows");
-    VerifyParams p{target, temperature == 0.f ? nullptr : draft, (long)target_sB, (long)target_sN, (long)draft_sB, (long)draft_sN, drafted,
-                   n_drafted, uniforms, B, N, V, temperature == 0.f ? 0.0 : 1.0 / (double)temperature, probs, accepted, tokens};
-    if (dtype == UW_DTYPE_F32) hipLaunchKernelGGL(verify_kernel<float>, dim3(B), dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(verify_kernel<bf16_t>, dim3(B), dim3(256), 0, (hipStream_t)stream, p);
+    const int rc = check_verify(a);
+    if (rc) return rc;
+    const bool greedy = a->temperature == 0.f;
+    VerifyParams p{a->target, greedy ? nullptr : a->draft, (long)a->target_sB, (long)a->target_sN, (long)a->draft_sB, (long)a->draft_sN,
+                   a->drafted, a->n_drafted, a->uniforms, a->B, a->N, a->V, greedy ? 0.0 : 1.0 / (double)a->temperature, a->probs,
+                   a->accepted, a->tokens};
+    if (a->dtype == UW_DTYPE_F32) hipLaunchKernelGGL(verify_kernel<float>, dim3(a->B), dim3(256), 0, (hipStream_t)stream, p);
+    else hipLaunchKernelGGL(verify_kernel<bf16_t>, dim3(a->B), dim3(256), 0, (hipStream_t)stream, p);
     UW_LAUNCH_CHECK();
     return UW_OK;
 }

@@ -28,16 +28,6 @@ class UwConfig(C.Structure):
     ]
 
 
-class UwKv8Cache(C.Structure):
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n_pages", C.c_int32),
-                ("n_kv_heads", C.c_int32), ("page", C.c_int32), ("head_dim", C.c_int32), ("format", C.c_int32)]
-
-
-class UwKv8Tokens(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_int64), ("tok_stride", C.c_int64), ("head_stride", C.c_int64),
-                ("n_tok", C.c_int64), ("tok_start", C.c_void_p), ("B", C.c_int32), ("T", C.c_int32)]
-
-
 class UwError(RuntimeError):
     pass
 
@@ -71,16 +61,13 @@ SIGNATURES = {
     "uw_profile_begin": (C.c_int, [_vp, C.c_int]),
     "uw_profile_end": (C.c_int, [_vp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64), C.POINTER(C.c_double)]),
     "uw_profile_span": (C.c_int, [_vp, C.c_int, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(C.c_double)]),
-    "uw_kv8_append": (C.c_int, [C.POINTER(UwKv8Cache), C.c_int, C.POINTER(UwKv8Tokens), C.POINTER(UwKv8Tokens), _vp, C.c_int,
-                                _vp, _vp]),
-    "uw_kv8_read": (C.c_int, [C.POINTER(UwKv8Cache), C.c_int, C.POINTER(UwKv8Tokens), C.POINTER(UwKv8Tokens), _vp, C.c_int,
-                              _vp, _vp]),
-    "uw_kv8_attention_workspace_bytes": (_i64, [C.POINTER(UwKv8Cache), C.c_int, C.c_int, _i64, C.c_int, C.c_int]),
-    "uw_kv8_attention": (C.c_int, [C.POINTER(UwKv8Cache), C.c_int, C.POINTER(UwKv8Tokens), C.POINTER(UwKv8Tokens), _vp, C.c_int,
-                                   _vp, C.c_int, _vp, C.c_int, C.c_float, _vp, _vp]),
-    "uw_verify_draft_workspace_bytes": (_i64, [C.c_int, C.c_int, C.c_int]),
-    "uw_verify_draft": (C.c_int, [C.c_int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_float,
-                                  C.c_int, _vp, _vp, _vp, _vp]),
+    # these take one structure, packed by the caller (kv8.py, speculative.py)
+    "uw_kv8_append": (C.c_int, [C.c_char_p, _vp]),
+    "uw_kv8_read": (C.c_int, [C.c_char_p, _vp]),
+    "uw_kv8_attention_workspace_bytes": (_i64, [C.c_char_p]),
+    "uw_kv8_attention": (C.c_int, [C.c_char_p, _vp]),
+    "uw_verify_draft_workspace_bytes": (_i64, [C.c_char_p]),
+    "uw_verify_draft": (C.c_int, [C.c_char_p, _vp]),
 }
 
 _lib: Optional[C.CDLL] = None

@@ -3,13 +3,22 @@ uw_verify_draft in include/uw_hip.h).  The scores are what `Engine.decoder_forwa
 positions: one pass of the decoder scores all of them."""
 from __future__ import annotations
 
+from struct import Struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import lib as L
+from .kv8 import _call
 
 _DTYPES = {torch.float32: L.UW_DTYPE_F32, torch.bfloat16: L.UW_DTYPE_BF16}
+_ARGS = Struct("@P2q P2q 5P Pq 4ifi")          # uw_verify_args
+
+
+def _ints(x: torch.Tensor, shape, what: str, dev: int) -> torch.Tensor:
+    if x.shape != shape or x.dtype not in (torch.int32, torch.int64) or x.get_device() != dev:
+        raise ValueError(f"{what} must be int32 {list(shape)} beside target, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
 
 
 def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: Optional[torch.Tensor] = None,
@@ -25,46 +34,47 @@ def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: Optional
 
     Returns accepted i32 [B] and tokens i32 [B, N + 1]: the accepted tokens, then the next token, then -1.  The tokens are
     distributed as if drawn from the target alone.  A next token of -1 says that its row held a NaN or no mass."""
-    if target.dim() != 3 or target.dtype not in _DTYPES:
-        raise ValueError(f"target must be float32 or bfloat16 [B, N + 1, V], got {target.dtype} {tuple(target.shape)}")
-    B, rows, V = target.shape
-    N, dev = rows - 1, target.device
-    if B == 0 or rows == 0 or V == 0:
-        raise ValueError(f"empty target {tuple(target.shape)}")
+    shape = target.shape
+    if len(shape) != 3 or target.dtype not in _DTYPES:
+        raise ValueError(f"target must be float32 or bfloat16 [B, N + 1, V], got {target.dtype} {tuple(shape)}")
+    if 0 in shape:
+        raise ValueError(f"empty target {tuple(shape)}")
+    B, N, V = shape[0], shape[1] - 1, shape[2]
+    dev = target.get_device()
     if not 0.0 <= temperature < float("inf"):
         raise ValueError(f"temperature must be finite and not negative, got {temperature}")
-    if probs and temperature not in (0.0, 1.0):
+    greedy = temperature == 0.0
+    if probs and not greedy and temperature != 1.0:
         raise ValueError("probabilities take no temperature: apply it before the softmax")
-    if drafted.shape != (B, N) or drafted.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"drafted must be int32 [{B}, {N}], got {drafted.dtype} {tuple(drafted.shape)}")
-    if draft is not None and (draft.shape != (B, N, V) or draft.dtype != target.dtype):
-        raise ValueError(f"draft must be {target.dtype} [{B}, {N}, {V}], got {draft.dtype} {tuple(draft.shape)}")
-    if temperature > 0.0 and (uniforms is None or uniforms.shape != (B, N + 1) or uniforms.dtype != torch.float32):
-        raise ValueError(f"uniforms must be float32 [{B}, {N + 1}]")
-    if n_drafted is not None and (n_drafted.shape != (B,) or n_drafted.dtype not in (torch.int32, torch.int64)):
-        raise ValueError(f"n_drafted must be int32 [{B}]")
-    for name, t in (("drafted", drafted), ("uniforms", uniforms), ("draft", draft), ("n_drafted", n_drafted)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, target on {dev}")
-    if not target.is_cuda:
-        raise L.UwError("target is not on a GPU: this operator runs on MI355X only (no CPU fallback)")
-    if target.stride(2) != 1:
-        target = target.contiguous()
-    if draft is not None and draft.stride(2) != 1:
-        draft = draft.contiguous()
-    drafted = drafted.to(torch.int32).contiguous()
-    if uniforms is not None:
-        uniforms = uniforms.contiguous()
+    drafted = _ints(drafted, (B, N), "drafted", dev)
     if n_drafted is not None:
-        n_drafted = n_drafted.to(torch.int32).contiguous()
-    accepted = torch.empty((B,), dtype=torch.int32, device=dev)
-    tokens = torch.empty((B, N + 1), dtype=torch.int32, device=dev)
+        n_drafted = _ints(n_drafted, (B,), "n_drafted", dev)
+    if draft is not None:
+        if draft.shape != (B, N, V) or draft.dtype != target.dtype or draft.get_device() != dev:
+            raise ValueError(f"draft must be {target.dtype} [{B}, {N}, {V}] beside target, got {draft.dtype} {tuple(draft.shape)} on {draft.device}")
+        if draft.stride(2) != 1:
+            draft = draft.contiguous()
+    if not greedy:
+        if uniforms is None or uniforms.shape != (B, N + 1) or uniforms.dtype != torch.float32 or uniforms.get_device() != dev:
+            raise ValueError(f"uniforms must be float32 [{B}, {N + 1}] beside target")
+        uniforms = uniforms.contiguous()
+    if dev < 0:
+        raise L.UwError("target is not on a GPU: this operator runs on MI355X only (no CPU fallback)")
+    st = target.stride()
+    if st[2] != 1:
+        target = target.contiguous()
+        st = target.stride()
+    accepted, tokens = drafted.new_empty(B), drafted.new_empty((B, N + 1))
     lib = L.load()
-    need = lib.uw_verify_draft_workspace_bytes(B, N, V)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    ds = draft.stride() if draft is not None else (0, 0, 0)
-    with torch.cuda.device(dev):
-        L.check(lib.uw_verify_draft(_DTYPES[target.dtype], target.data_ptr(), target.stride(0), target.stride(1), L.ptr(draft), ds[0], ds[1],
-                                    drafted.data_ptr(), L.ptr(n_drafted), L.ptr(uniforms), B, N, V, float(temperature), int(probs),
-                                    accepted.data_ptr(), tokens.data_ptr(), L.ptr(ws), L.stream_handle()))
+    use_draft = draft is not None and not greedy
+    head = (target.data_ptr(), st[0], st[1], draft.data_ptr() if use_draft else 0, *(draft.stride()[:2] if use_draft else (0, 0)),
+            drafted.data_ptr(), 0 if n_drafted is None else n_drafted.data_ptr(), 0 if greedy else uniforms.data_ptr(), accepted.data_ptr(),
+            tokens.data_ptr())
+    tail = (_DTYPES[target.dtype], B, N, V, temperature, 1 if probs else 0)
+    args = _ARGS.pack(*head, 0, 0, *tail)
+    need = lib.uw_verify_draft_workspace_bytes(args)
+    if need > 0:
+        ws = drafted.new_empty((need + 3) // 4)
+        args = _ARGS.pack(*head, ws.data_ptr(), need, *tail)
+    _call(lib.uw_verify_draft, args, dev)
     return accepted, tokens
