@@ -129,4 +129,9 @@ def test_verify_draft_refuses():
         args = _ARGS.pack(*{**good, **kw}.values())
         assert lib.uw_verify_draft(args, None) > 0 and word.encode() in lib.uw_last_error(), (kw, lib.uw_last_error())
         assert lib.uw_verify_draft_workspace_bytes(args) == -1
+    args = _ARGS.pack(*good.values())
+    assert lib.uw_verify_draft_workspace_bytes(args) > 0
+    for ws in (dict(), dict(ws=72, ws_bytes=1 << 20), dict(ws=64, ws_bytes=16)):
+        assert lib.uw_verify_draft(_ARGS.pack(*{**good, **ws}.values()), None) > 0 and b"workspace" in lib.uw_last_error()
+    assert lib.uw_verify_draft(_ARGS.pack(*{**good, "B": 1 << 20, "V": 51865}.values()), None) > 0 and b"too many rows" in lib.uw_last_error()
     assert lib.uw_verify_draft(None, None) > 0

@@ -1,7 +1,16 @@
 // Verification of drafted tokens against the target model's scores (speculative decoding), from given random numbers.
 //
+//   p_i = softmax(target_i / T), q_i = softmax(draft_i / T);  token i stands while u_i q_i(d_i) < p_i(d_i);  at the first that does
+//   not, the next token comes from max(p_i - q_i, 0), otherwise from p_n: the first index whose cumulative weight exceeds u_N sum w.
+//
 // Everything that decides about a token is held in 64 bits: a cumulative sum over a vocabulary of 50 000 has a border every 2e-5 on
 // average, and in 32 bits (1e-7 a step) about one draw in a hundred would fall on the wrong side of one.
+//
+// A vocabulary row is cut into chunks of 4096 scores, 16 to a thread, and three launches follow the data: (1) maximum and sum of
+// exponentials of every chunk of every row -- the one pass over all scores, bound by HBM; (2) each chunk's workgroup joins the
+// rows' statistics, decides how many tokens stand, and sums the weights of its chunk of the one row that is drawn from (which is
+// in L2 or the Infinity Cache by then); (3) a workgroup per sequence finds the chunk, then the token in it.  Probabilities need no
+// (1); greedy verification needs the arg-max of (1) and then one small launch.
 #include "../../include/uw_hip.h"
 #include "uw_common.h"
 #include "uw_kernels.h"
@@ -9,173 +18,376 @@
 
 namespace {
 
+constexpr int CHUNK = 4096, PER = 16;      // scores per workgroup and per thread
+
+struct ChunkStat { double z; float mx; int arg; };         // sum of exp((x - mx) / T), maximum, its lowest index (-1: a NaN, greedy only)
+struct Chosen { double zp, zq; float mp, mq; int acc, mode; };   // the rows drawn from; mode 0: p alone, 1: p - q, 2: p without the drafted token
+
 struct VerifyParams {
     const void *target, *draft;
     long t_sB, t_sN, d_sB, d_sN;
     const int32_t *drafted, *n_drafted;
     const float* u;
-    int B, N, V;
+    int B, N, V, chunks;
     double inv_t;
     int probs;
     int32_t *accepted, *tokens;
+    ChunkStat *t_stat, *d_stat;     // [B][N + 1][chunks], [B][N][chunks]
+    double* mass;                   // [B][chunks][2]: of the residual, of p
+    Chosen* chosen;                 // [B]
+
+    __device__ __forceinline__ int n_of(int b) const { return n_drafted ? min(max(n_drafted[b], 0), N) : N; }
 };
 
-__device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor(v, o, 64); }
+// exp(t) for t <= 0 (and NaN): 2^n e^r, |r| <= ln2 / 2, e^r by its series to r^11 (next term 6e-15 relative).  A dozen f64
+// instructions, against the library's table and special cases.
+__device__ __forceinline__ double exp_neg(double t)
+{
+    t = t < -800.0 ? -800.0 : t;
+    const double n = rint(t * 1.4426950408889634074);
+    double r = fma(n, -0.6931471824645996, t);      // ln 2 as its float, n times which is exact, and the rest
+    r = fma(n, 1.904654299957768e-09, r);
+    double y = 1.0 / 39916800.0;
+    y = fma(y, r, 1.0 / 3628800.0);
+    y = fma(y, r, 1.0 / 362880.0);
+    y = fma(y, r, 1.0 / 40320.0);
+    y = fma(y, r, 1.0 / 5040.0);
+    y = fma(y, r, 1.0 / 720.0);
+    y = fma(y, r, 1.0 / 120.0);
+    y = fma(y, r, 1.0 / 24.0);
+    y = fma(y, r, 1.0 / 6.0);
+    y = fma(y, r, 0.5);
+    y = fma(y, r, 1.0);
+    y = fma(y, r, 1.0);
+    return ldexp(y, (int)n);
+}
 
-// sum / max over a 256-thread workgroup, valid in all threads; scratch: 4 doubles
-__device__ __forceinline__ double block_sum_d(double v, double* s)
+// PER scores of a chunk: piece u of thread t begins at u * 256 * VEC + t * VEC; -inf behind the row's end.  Rows begin at any address
+// that a score may have, so the 16-byte loads assume no more.
+template <typename T> struct Piece;
+template <> struct Piece<float> { typedef float V __attribute__((ext_vector_type(4), aligned(4))); static constexpr int VEC = 4; };
+template <> struct Piece<bf16_t> { typedef unsigned short V __attribute__((ext_vector_type(8), aligned(2))); static constexpr int VEC = 8; };
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
+
+template <typename T> __device__ __forceinline__ int score_index(int j0, int k)
+{
+    constexpr int VEC = Piece<T>::VEC;
+    return j0 + (k / VEC) * 256 * VEC + (int)threadIdx.x * VEC + k % VEC;
+}
+template <typename T> __device__ __forceinline__ void load_scores(const T* row, int j0, int V, float* x, float fill)
+{
+    constexpr int VEC = Piece<T>::VEC;
+#pragma unroll
+    for (int u = 0; u < PER / VEC; ++u) {
+        const int j = score_index<T>(j0, u * VEC);
+        if (j + VEC <= V) {
+            const typename Piece<T>::V v = *(const typename Piece<T>::V*)(row + j);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[u * VEC + e] = widen(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[u * VEC + e] = j + e < V ? to_f32<T>(row[j + e]) : fill;
+        }
+    }
+}
+
+__device__ __forceinline__ double wave_sum_d(double v)
 {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += shfl_xor_d(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (s[0] + s[1]) + (s[2] + s[3]);
-}
-__device__ __forceinline__ float block_max_f(float v, double* s)
-{
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (float)fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
-struct RowStat { float mx; double z; };
-
-template <typename T> __device__ RowStat row_stat(const VerifyParams& p, const T* row, double* s)
+// (1) grid (chunks, B * (N + 1) target rows, then B * N draft rows)
+template <typename T, bool GREEDY>
+__global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p)
 {
+    __shared__ double s_z[4];
+    __shared__ float s_m[4];
+    __shared__ int s_a[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int c = blockIdx.x % p.chunks;
+    int row = blockIdx.x / p.chunks;
+    const bool is_draft = row >= p.B * (p.N + 1);
+    if (is_draft) row -= p.B * (p.N + 1);
+    const int per = is_draft ? p.N : p.N + 1, b = row / per, i = row % per;
+    if (i > p.n_of(b) - (is_draft ? 1 : 0)) return;                // no token there: nothing reads its statistics
+    const T* x0 = is_draft ? (const T*)p.draft + (long)b * p.d_sB + (long)i * p.d_sN : (const T*)p.target + (long)b * p.t_sB + (long)i * p.t_sN;
+    const int j0 = c * CHUNK;
+    float x[PER];
+    load_scores<T>(x0, j0, p.V, x, -INFINITY);
     float mx = -INFINITY;
-    bool bad = false;
-    for (int j = threadIdx.x; j < p.V; j += 256) {
-        const float x = to_f32<T>(row[j]);
-        bad |= x != x;
-        mx = fmaxf(mx, x);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) mx = fmaxf(mx, x[k]);
+    mx = wave_max(mx);
+    if (lane == 0) s_m[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    ChunkStat* out = (is_draft ? p.d_stat : p.t_stat) + (long)row * p.chunks + c;
+    if constexpr (GREEDY) {
+        int arg = 0x7fffffff;
+        bool bad = false;
+#pragma unroll
+        for (int k = PER - 1; k >= 0; --k) {
+            if (x[k] == mx) arg = score_index<T>(j0, k);            // a thread's indexes ascend with k
+            bad |= x[k] != x[k];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
+        if (lane == 0) s_a[wave] = arg;
+        bad = __syncthreads_or(bad);
+        if (tid == 0) *out = ChunkStat{0.0, mx, bad ? -1 : min(min(s_a[0], s_a[1]), min(s_a[2], s_a[3]))};
+    } else {
+        const double base = mx == -INFINITY ? 0.0 : (double)mx;
+        double z = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) z += exp_neg(((double)x[k] - base) * p.inv_t);
+        z = wave_sum_d(z);
+        if (lane == 0) s_z[wave] = z;
+        __syncthreads();
+        if (tid == 0) *out = ChunkStat{(s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), mx, 0};
     }
-    bad = __syncthreads_or(bad);
-    mx = block_max_f(mx, s);
-    if (bad) mx = __uint_as_float(0x7fc00000u);
-    double z = 0;
-    for (int j = threadIdx.x; j < p.V; j += 256) z += exp(((double)to_f32<T>(row[j]) - (double)mx) * p.inv_t);
-    return RowStat{mx, block_sum_d(z, s)};
-}
-template <typename T> __device__ __forceinline__ double prob(const VerifyParams& p, const T* row, int j, const RowStat& st)
-{
-    const double x = to_f32<T>(row[j]);
-    return p.probs ? x : exp((x - (double)st.mx) * p.inv_t) / st.z;
 }
 
-// one workgroup per sequence
-template <typename T>
-__global__ __launch_bounds__(256) void verify_kernel(VerifyParams p)
+// maximum and sum of a whole row from its chunks; one wave, the same in all lanes and -- the order being fixed -- in all workgroups
+__device__ __forceinline__ void join_row(const ChunkStat* st, int chunks, double inv_t, float& m, double& z)
 {
-    __shared__ double s[4];
-    __shared__ double cum[256];
-    __shared__ int s_i[4];
-    const int b = blockIdx.x, tid = threadIdx.x;
-    const int n = p.n_drafted ? min(max(p.n_drafted[b], 0), p.N) : p.N;
+    const int lane = threadIdx.x & 63;
+    m = -INFINITY;
+    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, st[c].mx);
+    m = wave_max(m);
+    z = 0;
+    for (int c = lane; c < chunks; c += 64) {
+        const ChunkStat s = st[c];
+        z += s.mx == -INFINITY ? s.z : s.z * exp_neg(((double)s.mx - (double)m) * inv_t);    // (z of a chunk of -inf is 0, or NaN)
+    }
+    z = wave_sum_d(z);
+}
+
+// (2) grid (chunks, B)
+template <typename T>
+__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
+{
+    __shared__ int s_ok[4];
+    __shared__ double s_z[4], s_r[4];
+    __shared__ float s_m[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x % p.chunks, b = blockIdx.x / p.chunks;
+    const int n = p.n_of(b), V = p.V;
     const T* tb = (const T*)p.target + (long)b * p.t_sB;
     const T* db = p.draft ? (const T*)p.draft + (long)b * p.d_sB : nullptr;
     const int32_t* d = p.drafted + (long)b * p.N;
-    const float* u = p.u + (long)b * (p.N + 1);
-    int acc = 0, next = -1;
-    if (p.inv_t == 0.0) {
-        for (;; ++acc) {
-            const T* row = tb + (long)acc * p.t_sN;
-            float best = -INFINITY;
-            int arg = 0x7fffffff;
-            bool bad = false;
-            for (int j = tid; j < p.V; j += 256) {
-                const float x = to_f32<T>(row[j]);
-                bad |= x != x;
-                if (x > best || (x == best && j < arg)) { best = x; arg = j; }
-            }
-            bad = __syncthreads_or(bad);
-            const float top = block_max_f(best, s);
-            int cand = best == top ? arg : 0x7fffffff;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) cand = min(cand, __shfl_xor(cand, o, 64));
-            if ((tid & 63) == 0) s_i[tid >> 6] = cand;
-            __syncthreads();
-            next = min(min(s_i[0], s_i[1]), min(s_i[2], s_i[3]));
-            __syncthreads();
-            if (bad) { next = -1; break; }
-            if (acc >= n || d[acc] != next) break;
-        }
-    } else {
-        RowStat ps{0.f, 1.0}, qs{0.f, 1.0};
-        for (; acc <= n; ++acc) {
-            const T* row = tb + (long)acc * p.t_sN;
-            if (!p.probs) ps = row_stat<T>(p, row, s);
-            if (acc == n) break;
-            const int di = d[acc];
-            if (di < 0 || di >= p.V) break;
+    const ChunkStat* ts = p.t_stat + (long)b * (p.N + 1) * p.chunks;
+    const ChunkStat* ds = p.d_stat + (long)b * p.N * p.chunks;
+    const auto probability = [&](float x, float m, double z) { return p.probs ? (double)x : exp_neg(((double)x - (double)m) * p.inv_t) / z; };
+
+    // how many tokens stand: four at a time, a wave each
+    int acc = 0;
+    for (int i0 = 0; i0 < n; i0 += 4) {
+        const int i = i0 + wave;
+        bool ok = false;
+        if (i < n && d[i] >= 0 && d[i] < V) {
+            float m = 0;
+            double z = 1;
+            if (!p.probs) join_row(ts + (long)i * p.chunks, p.chunks, p.inv_t, m, z);
+            const double pd = probability(to_f32<T>(tb[(long)i * p.t_sN + d[i]]), m, z);
             double qd = 1.0;
             if (db) {
-                const T* qrow = db + (long)acc * p.d_sN;
-                if (!p.probs) qs = row_stat<T>(p, qrow, s);
-                qd = prob<T>(p, qrow, di, qs);
+                if (!p.probs) join_row(ds + (long)i * p.chunks, p.chunks, p.inv_t, m, z);
+                qd = probability(to_f32<T>(db[(long)i * p.d_sN + d[i]]), m, z);
             }
-            if (!((double)u[acc] * qd < prob<T>(p, row, di, ps))) break;
+            ok = (double)p.u[(long)b * (p.N + 1) + i] * qd < pd;
         }
-        const T* row = tb + (long)acc * p.t_sN;
-        const T* qrow = (db && acc < n) ? db + (long)acc * p.d_sN : nullptr;
-        if (qrow && !p.probs) qs = row_stat<T>(p, qrow, s);
-        const int point = (acc < n && !db) ? d[acc] : -1;
-        // thread t owns a contiguous run of the vocabulary
-        const int per = (p.V + 255) / 256, j0 = min(tid * per, p.V), j1 = min(j0 + per, p.V);
-        bool residual = qrow || point >= 0;
-        for (;;) {
-            auto weight = [&](int j) {
-                double w = prob<T>(p, row, j, ps);
-                if (residual) {
-                    if (j == point) w = 0;
-                    else if (qrow) { const double dq = prob<T>(p, qrow, j, qs); w = (w != w || dq != dq) ? w + dq : fmax(w - dq, 0.0); }
-                }
-                return w;
-            };
-            double sum = 0;
-            for (int j = j0; j < j1; ++j) sum += weight(j);
-            __syncthreads();
-            cum[tid] = sum;
-            __syncthreads();
-            if (tid == 0)
-                for (int i = 1; i < 256; ++i) cum[i] += cum[i - 1];
-            if (tid == 0) s_i[0] = -1;
-            __syncthreads();
-            const double total = cum[255];
-            if (!(total > 0.0) && !(total != total) && residual) { residual = false; continue; }
-            if (!(total > 0.0) || !(total < INFINITY)) break;
-            const double r = (double)u[p.N] * total;
-            const double before = tid ? cum[tid - 1] : 0.0;
-            // the first thread whose cumulative weight exceeds r holds the token; rounding may leave none: then the last with mass
-            const bool holds = cum[tid] > r && !(before > r);
-            int found = -1, last = -1;
-            double c = before;
-            if (sum > 0)
-                for (int j = j0; j < j1; ++j) {
-                    const double w = weight(j);
-                    c += w;
-                    if (w > 0) last = j;
-                    if (holds && found < 0 && c > r) found = j;
-                }
-            if (holds && found < 0) found = last;
-            if (holds) s_i[0] = found;
-            __syncthreads();
-            next = s_i[0];
-            if (next < 0) {
+        if (lane == 0) s_ok[wave] = ok;
+        __syncthreads();
+        const int run = !s_ok[0] ? 0 : !s_ok[1] ? 1 : !s_ok[2] ? 2 : !s_ok[3] ? 3 : 4;
+        __syncthreads();
+        acc = i0 + run;
+        if (run < 4) break;
+    }
+    acc = min(acc, n);
+
+    // the rows that the next token is drawn from
+    const T* row = tb + (long)acc * p.t_sN;
+    const T* qrow = (db && acc < n) ? db + (long)acc * p.d_sN : nullptr;
+    const int point = (!db && acc < n && d[acc] >= 0 && d[acc] < V) ? d[acc] : -1;
+    if (!p.probs && (wave == 0 || (wave == 1 && qrow))) {
+        float m;
+        double z;
+        join_row(wave ? ds + (long)acc * p.chunks : ts + (long)acc * p.chunks, p.chunks, p.inv_t, m, z);
+        if (lane == 0) { s_m[wave] = m; s_z[wave] = z; }
+    }
+    __syncthreads();
+    const float mp = p.probs ? 0.f : s_m[0], mq = (p.probs || !qrow) ? 0.f : s_m[1];
+    const double zp = p.probs ? 1.0 : s_z[0], zq = (p.probs || !qrow) ? 1.0 : s_z[1];
+    __syncthreads();
+
+    float x[PER], y[PER];
+    const int j0 = c * CHUNK;
+    const float none = p.probs ? 0.f : -INFINITY;
+    load_scores<T>(row, j0, V, x, none);
+    if (qrow) load_scores<T>(qrow, j0, V, y, none);
+    double sp = 0, sr = 0;
 #pragma unroll
-                for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
-                __syncthreads();
-                if ((tid & 63) == 0) s_i[tid >> 6] = last;
-                __syncthreads();
-                next = max(max(s_i[0], s_i[1]), max(s_i[2], s_i[3]));
-            }
-            break;
+    for (int k = 0; k < PER; ++k) {
+        const double w = probability(x[k], mp, zp);
+        sp += w;
+        if (qrow) {
+            const double r = w - probability(y[k], mq, zq);
+            sr += r != r ? r : fmax(r, 0.0);
+        } else if (score_index<T>(j0, k) != point) {
+            sr += w;
         }
     }
-    if (tid == 0) p.accepted[b] = acc;
-    for (int i = tid; i <= p.N; i += 256) p.tokens[(long)b * (p.N + 1) + i] = i < acc ? d[i] : i == acc ? next : -1;
+    sp = wave_sum_d(sp);
+    sr = wave_sum_d(sr);
+    if (lane == 0) { s_z[wave] = sp; s_r[wave] = sr; }
+    __syncthreads();
+    if (tid == 0) {
+        double* at = p.mass + ((long)b * p.chunks + c) * 2;
+        at[0] = (s_r[0] + s_r[1]) + (s_r[2] + s_r[3]);
+        at[1] = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
+        if (c == 0) p.chosen[b] = Chosen{zp, zq, mp, mq, acc, qrow ? 1 : point >= 0 ? 2 : 0};
+    }
+}
+
+// the answer of one sequence
+__device__ __forceinline__ void write_tokens(const VerifyParams& p, int b, int acc, int next)
+{
+    if (threadIdx.x == 0) p.accepted[b] = acc;
+    for (int i = threadIdx.x; i <= p.N; i += blockDim.x)
+        p.tokens[(long)b * (p.N + 1) + i] = i < acc ? p.drafted[(long)b * p.N + i] : i == acc ? next : -1;
+}
+
+// (3) grid B: which chunk, then which token
+template <typename T>
+__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
+{
+    __shared__ double s_c[256];
+    __shared__ double s_r;
+    __shared__ int s_chunk, s_next, s_last[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+    const Chosen ch = p.chosen[b];
+    const double* mass = p.mass + (long)b * p.chunks * 2;
+    // totals of the residual and of p, over the chunks in order
+    double tot[2] = {0, 0};
+    for (int c0 = 0; c0 < p.chunks; c0 += 128) {
+        __syncthreads();
+        if (c0 + (tid >> 1) < p.chunks) s_c[tid] = mass[(long)c0 * 2 + tid];
+        __syncthreads();
+        for (int c = 0; c < min(128, p.chunks - c0); ++c) { tot[0] += s_c[2 * c]; tot[1] += s_c[2 * c + 1]; }
+    }
+    // an empty residual (probabilities that do not add up alike) leaves the row itself
+    const int which = (ch.mode == 0 || tot[0] == 0.0) ? 1 : 0;
+    const double total = tot[which];
+    if (!(total > 0.0 && total < INFINITY)) { write_tokens(p, b, ch.acc, -1); return; }
+    const double r = (double)p.u[(long)b * (p.N + 1) + p.N] * total;
+    if (tid == 0) {
+        // the first chunk whose cumulative weight exceeds r; if rounding leaves none, the last one with weight
+        double cum = 0, before = 0;
+        int at = -1, last = 0;
+        double last_before = 0;
+        for (int c = 0; c < p.chunks; ++c) {
+            const double w = mass[2 * c + which];
+            if (w > 0) { last = c; last_before = cum; }
+            if (cum + w > r) { at = c; before = cum; break; }
+            cum += w;
+        }
+        s_chunk = at < 0 ? last : at;
+        s_r = r - (at < 0 ? last_before : before);
+        s_next = 0x7fffffff;
+    }
+    __syncthreads();
+    const int j0 = s_chunk * CHUNK, V = p.V, b0 = j0 + tid * PER;
+    const T* row = (const T*)p.target + (long)b * p.t_sB + (long)ch.acc * p.t_sN;
+    const T* qrow = (const T*)p.draft + (long)b * p.d_sB + (long)ch.acc * p.d_sN;
+    const int mode = which ? 0 : ch.mode, point = mode == 2 ? p.drafted[(long)b * p.N + ch.acc] : -1;
+    // a thread's 16 scores follow one another here, so that its weights can be added up in order
+    double w[PER], sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int j = b0 + k;
+        double v = 0;
+        if (j < V) {
+            v = p.probs ? (double)to_f32<T>(row[j]) : exp_neg(((double)to_f32<T>(row[j]) - (double)ch.mp) * p.inv_t) / ch.zp;
+            if (mode == 1) v = fmax(v - (p.probs ? (double)to_f32<T>(qrow[j]) : exp_neg(((double)to_f32<T>(qrow[j]) - (double)ch.mq) * p.inv_t) / ch.zq), 0.0);
+            if (j == point) v = 0;
+        }
+        w[k] = v;
+        sum += v;
+    }
+    double incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 63) s_c[wave] = incl;
+    __syncthreads();
+    for (int k = 0; k < wave; ++k) incl += s_c[k];
+    double cum = incl - sum;
+    int found = 0x7fffffff, last = -1;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        cum += w[k];
+        if (w[k] > 0) last = b0 + k;
+        if (w[k] > 0 && cum > s_r) found = min(found, b0 + k);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        found = min(found, __shfl_xor(found, o, 64));
+        last = max(last, __shfl_xor(last, o, 64));
+    }
+    if (lane == 0) { s_last[wave] = last; atomicMin(&s_next, found); }      // (a minimum: the order of arrival is nothing to it)
+    __syncthreads();
+    const int next = s_next != 0x7fffffff ? s_next : max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
+    write_tokens(p, b, ch.acc, next);
+}
+
+// greedy: grid B
+__global__ __launch_bounds__(256) void verify_greedy_kernel(VerifyParams p)
+{
+    __shared__ int s_a[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x, n = p.n_of(b);
+    const ChunkStat* ts = p.t_stat + (long)b * (p.N + 1) * p.chunks;
+    int acc = 0, next = -1;
+    for (int i0 = 0;; i0 += 4) {
+        const int i = i0 + wave;
+        int arg = 0x7fffffff;
+        if (i <= n) {
+            float m = -INFINITY;
+            bool bad = false;
+            for (int c = lane; c < p.chunks; c += 64) {
+                const ChunkStat s = ts[(long)i * p.chunks + c];
+                bad |= s.arg < 0;
+                if (s.mx > m || arg == 0x7fffffff) { m = s.mx; arg = s.arg; }      // chunks ascend: the first of equal ones stays
+            }
+            const float top = wave_max(m);
+            if (m != top) arg = 0x7fffffff;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
+            if (__any(bad)) arg = -1;
+        }
+        if (lane == 0) s_a[wave] = arg;
+        __syncthreads();
+        int w = 0;
+        for (; w < 4; ++w) {
+            next = s_a[w];
+            acc = i0 + w;
+            if (acc >= n || next < 0 || next != p.drafted[(long)b * p.N + acc]) break;
+        }
+        __syncthreads();
+        if (w < 4) break;
+    }
+    write_tokens(p, b, acc, next);
+}
+
+long chunks_of(const uw_verify_args* a) { return ceil_div(a->V, CHUNK); }
+bool all_rows(const uw_verify_args* a) { return !a->probs || a->temperature == 0.f; }
+int64_t workspace_bytes(const uw_verify_args* a)
+{
+    const int64_t rows = all_rows(a) ? (int64_t)a->B * (a->N + 1 + (a->temperature > 0.f && a->draft ? a->N : 0)) : 0;
+    return rows * chunks_of(a) * (int64_t)sizeof(ChunkStat) + (int64_t)a->B * (chunks_of(a) * 16 + (int64_t)sizeof(Chosen));
 }
 
 int check_verify(const uw_verify_args* a)
@@ -183,6 +395,7 @@ int check_verify(const uw_verify_args* a)
     UW_REQUIRE(a, "uw_verify_draft: null arguments");
     UW_REQUIRE(a->dtype == UW_DTYPE_F32 || a->dtype == UW_DTYPE_BF16, "uw_verify_draft: dtype must be f32 or bf16");
     UW_REQUIRE(a->B > 0 && a->N >= 0 && a->V > 0, "uw_verify_draft: B %d, N %d, V %d", a->B, a->N, a->V);
+    UW_REQUIRE(a->V <= 0x7fffffff - CHUNK && (double)a->B * (2.0 * a->N + 1) * ((a->V + CHUNK - 1) / CHUNK) < (1 << 24), "uw_verify_draft: too many rows");
     UW_REQUIRE(a->target && a->accepted && a->tokens && (a->drafted || a->N == 0), "uw_verify_draft: null argument");
     UW_REQUIRE(a->temperature >= 0.f && a->temperature < INFINITY, "uw_verify_draft: temperature must be finite and not negative");
     UW_REQUIRE(a->uniforms || a->temperature == 0.f, "uw_verify_draft: uniforms missing");
@@ -195,18 +408,59 @@ int check_verify(const uw_verify_args* a)
 
 extern "C" {
 
-int64_t uw_verify_draft_workspace_bytes(const uw_verify_args* a) { return check_verify(a) ? -1 : 0; }
+int64_t uw_verify_draft_workspace_bytes(const uw_verify_args* a) { return check_verify(a) ? -1 : workspace_bytes(a); }
 
 int uw_verify_draft(const uw_verify_args* a, void* stream)
 {
     const int rc = check_verify(a);
     if (rc) return rc;
+    UW_REQUIRE(a->ws && ((uintptr_t)a->ws & 15) == 0 && a->ws_bytes >= workspace_bytes(a),
+               "uw_verify_draft: workspace missing, misaligned or smaller than %lld bytes", (long long)workspace_bytes(a));
     const bool greedy = a->temperature == 0.f;
-    VerifyParams p{a->target, greedy ? nullptr : a->draft, (long)a->target_sB, (long)a->target_sN, (long)a->draft_sB, (long)a->draft_sN,
-                   a->drafted, a->n_drafted, a->uniforms, a->B, a->N, a->V, greedy ? 0.0 : 1.0 / (double)a->temperature, a->probs,
-                   a->accepted, a->tokens};
-    if (a->dtype == UW_DTYPE_F32) hipLaunchKernelGGL(verify_kernel<float>, dim3(a->B), dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(verify_kernel<bf16_t>, dim3(a->B), dim3(256), 0, (hipStream_t)stream, p);
+    const long chunks = chunks_of(a), t_rows = (long)a->B * (a->N + 1), d_rows = !greedy && a->draft ? (long)a->B * a->N : 0;
+    VerifyParams p;
+    p.target = a->target;
+    p.draft = greedy ? nullptr : a->draft;
+    p.t_sB = a->target_sB;
+    p.t_sN = a->target_sN;
+    p.d_sB = a->draft_sB;
+    p.d_sN = a->draft_sN;
+    p.drafted = a->drafted;
+    p.n_drafted = a->n_drafted;
+    p.u = a->uniforms;
+    p.B = a->B;
+    p.N = a->N;
+    p.V = a->V;
+    p.chunks = (int)chunks;
+    p.inv_t = greedy ? 0.0 : 1.0 / (double)a->temperature;
+    p.probs = a->probs;
+    p.accepted = a->accepted;
+    p.tokens = a->tokens;
+    p.chosen = (Chosen*)a->ws;
+    p.mass = (double*)(p.chosen + a->B);
+    p.t_stat = (ChunkStat*)(p.mass + (long)a->B * chunks * 2);
+    p.d_stat = p.t_stat + t_rows * chunks;
+    const hipStream_t s = (hipStream_t)stream;
+    const bool f32 = a->dtype == UW_DTYPE_F32;
+    const dim3 rows((unsigned)(chunks * (t_rows + d_rows))), one(256);
+    if (greedy) {
+        if (f32) hipLaunchKernelGGL((verify_rows_kernel<float, true>), rows, one, 0, s, p);
+        else hipLaunchKernelGGL((verify_rows_kernel<bf16_t, true>), rows, one, 0, s, p);
+        hipLaunchKernelGGL(verify_greedy_kernel, dim3(a->B), one, 0, s, p);
+    } else {
+        const dim3 mass((unsigned)(chunks * a->B));
+        if (!a->probs) {
+            if (f32) hipLaunchKernelGGL((verify_rows_kernel<float, false>), rows, one, 0, s, p);
+            else hipLaunchKernelGGL((verify_rows_kernel<bf16_t, false>), rows, one, 0, s, p);
+        }
+        if (f32) {
+            hipLaunchKernelGGL(verify_mass_kernel<float>, mass, one, 0, s, p);
+            hipLaunchKernelGGL(verify_pick_kernel<float>, dim3(a->B), one, 0, s, p);
+        } else {
+            hipLaunchKernelGGL(verify_mass_kernel<bf16_t>, mass, one, 0, s, p);
+            hipLaunchKernelGGL(verify_pick_kernel<bf16_t>, dim3(a->B), one, 0, s, p);
+        }
+    }
     UW_LAUNCH_CHECK();
     return UW_OK;
 }
