@@ -46,17 +46,25 @@ template <int F> __device__ __forceinline__ float kv8_decode(uint8_t c);
 template <> __device__ __forceinline__ float kv8_decode<UW_KV8_INT8>(uint8_t c) { return (float)(int8_t)c; }
 template <> __device__ __forceinline__ float kv8_decode<UW_KV8_E4M3>(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
 
-// code of x under the reciprocal scale r.  int8: the 48-bit product is taken in f64, so that it is rounded once and the code is
-// the definition's whatever the order of evaluation; e4m3: r is a power of two, the f32 product is exact where it matters.
-template <int F> __device__ __forceinline__ uint8_t kv8_encode(float x, float r);
-template <> __device__ __forceinline__ uint8_t kv8_encode<UW_KV8_INT8>(float x, float r)
+// Codes of four values under the reciprocal scale r.  int8: the 48-bit product is taken in f64, so that it is rounded once and the
+// code is the definition's whatever the order of evaluation; e4m3: r is a power of two, the f32 product is exact where it matters.
+template <int F> __device__ __forceinline__ unsigned kv8_encode4(const float* x, float r);
+template <> __device__ __forceinline__ unsigned kv8_encode4<UW_KV8_INT8>(const float* x, float r)
 {
-    return (uint8_t)(int8_t)(int)fmin(fmax(rint((double)x * (double)r), -127.0), 127.0);
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int q = (int)rint((double)x[i] * (double)r);       // |product| < 128: r fits the block's largest value
+        w |= ((unsigned)max(-127, min(127, q)) & 255u) << (8 * i);
+    }
+    return w;
 }
-template <> __device__ __forceinline__ uint8_t kv8_encode<UW_KV8_E4M3>(float x, float r)
+template <> __device__ __forceinline__ unsigned kv8_encode4<UW_KV8_E4M3>(const float* x, float r)
 {
-    const float y = fminf(fmaxf(x * r, -448.f), 448.f);
-    return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = fminf(fmaxf(x[i] * r, -448.f), 448.f);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
 }
 
 // smallest e with 2^e >= v, v a positive normal number
