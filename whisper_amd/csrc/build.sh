@@ -8,7 +8,7 @@ JOBS=4
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _build
 pids=()
-for f in uw_api uw_gemm uw_elementwise uw_attention uw_decode uw_mel uw_align uw_kv8 uw_verify; do
+for f in uw_api uw_gemm uw_elementwise uw_attention uw_decode uw_mel uw_align uw_kv8 uw_kv8_attention uw_verify; do
   if [ ! -f _build/$f.o ] || [ $f.hip -nt _build/$f.o ] || [ uw_common.h -nt _build/$f.o ] || [ uw_kernels.h -nt _build/$f.o ] || [ uw_kv8.h -nt _build/$f.o ] || [ ../../include/uw_hip.h -nt _build/$f.o ]; then
     ( hipcc $FLAGS -c $f.hip -o _build/$f.o ) &
     pids+=($!)

@@ -88,3 +88,116 @@ template <int F> __device__ __forceinline__ int kv8_growth(float amax, float s)
     const double need = (double)amax / ((F == UW_KV8_INT8 ? 127.5 : 448.0) * (double)s);   // int8: 127.5 still rounds to within half a step of 127
     return need > 1.0 ? ceil_log2(need) : 0;
 }
+
+struct TokArg {
+    void* data;
+    long sB, sT, sH;
+};
+
+// The idx-th (sequence, part) pair of a call, parts counted over the sequences in order; false past the last one.  cnt(b) = parts of
+// sequence b.  Every wave works it out for itself: 256 sequences per step, four to a lane so that their lengths are asked for at
+// once, and one shuffle scan.
+template <typename CNT> __device__ __forceinline__ bool locate(int idx, int B, CNT cnt, int& b_out, int& j_out)
+{
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int b0 = 0; b0 < B; b0 += 256) {
+        const int first = b0 + lane * 4;
+        int n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = first + i < B ? cnt(first + i) : 0;
+        const int own = (n[0] + n[1]) + (n[2] + n[3]);
+        int incl = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += up;
+        }
+        const unsigned long long over = __ballot(base + incl > idx);
+        if (over) {
+            const int w = __ffsll((long long)over) - 1;
+            int j = idx - base - __shfl(incl - own, w, 64), b = b0 + w * 4;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int c = __shfl(n[i], w, 64);
+                if (b == b0 + w * 4 + i && j >= c) { j -= c; ++b; }
+            }
+            b_out = __builtin_amdgcn_readfirstlane(b);
+            j_out = __builtin_amdgcn_readfirstlane(j);
+            return true;
+        }
+        base += __shfl(incl, 63, 64);
+    }
+    return false;
+}
+
+// ---- host side: what every entry checks -----------------------------------------------------------------
+#define RUN(x)                   \
+    do {                         \
+        const int rc__ = (x);    \
+        if (rc__) return rc__;   \
+    } while (0)
+
+static inline int log2_page(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : page == 256 ? 8 : -1; }
+
+static inline int check_cache(const char* fn, const uw_kv8_cache* c)
+{
+    UW_REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale, "%s: null cache", fn);
+    UW_REQUIRE(c->format == UW_KV8_INT8 || c->format == UW_KV8_E4M3, "%s: unknown code format %d", fn, c->format);
+    UW_REQUIRE(log2_page(c->page) > 0, "%s: a page holds 16, 32, 64, 128 or 256 tokens, not %d", fn, c->page);
+    UW_REQUIRE(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim 64 or 128, not %d", fn, c->head_dim);
+    UW_REQUIRE(c->n_pages > 0 && c->n_kv_heads > 0 && c->n_kv_heads <= 65535, "%s: %d pages of %d heads", fn, c->n_pages, c->n_kv_heads);
+    UW_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0 && (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) == 0,
+               "%s: cache arrays must be 16-byte aligned (scales 4)", fn);
+    return UW_OK;
+}
+
+static inline int check_seqs(const char* fn, const uw_kv8_seqs* t)
+{
+    UW_REQUIRE(t->dtype == UW_DTYPE_F32 || t->dtype == UW_DTYPE_BF16, "%s: dtype must be f32 or bf16", fn);
+    UW_REQUIRE(t->B > 0 && t->n_tok >= 0, "%s: %d sequences, %lld rows", fn, t->B, (long long)t->n_tok);
+    UW_REQUIRE(t->tok_start || (t->T >= 0 && t->n_tok == (int64_t)t->B * t->T), "%s: %lld rows are not %d x %d", fn,
+               (long long)t->n_tok, t->B, t->T);
+    UW_REQUIRE(t->n_tok <= 0x7fffffff, "%s: too many rows", fn);
+    UW_REQUIRE(t->table && t->len && t->table_width > 0, "%s: null page table or lengths, or no columns", fn);
+    UW_REQUIRE(t->table_width <= (1 << 23), "%s: %d table columns", fn, t->table_width);
+    return UW_OK;
+}
+
+static inline int check_tokens(const char* fn, const char* what, const uw_kv8_tokens* t, const uw_kv8_seqs* q)
+{
+    const int unit = q->dtype == UW_DTYPE_F32 ? 4 : 8;      // elements in 16 bytes
+    UW_REQUIRE(q->n_tok == 0 || t->data, "%s: %s: null data", fn, what);
+    UW_REQUIRE(((uintptr_t)t->data & 15) == 0 && t->seq_stride % unit == 0 && t->tok_stride % unit == 0 && t->head_stride % unit == 0,
+               "%s: %s: base and strides must be multiples of 16 bytes", fn, what);
+    return UW_OK;
+}
+
+static inline Kv8View view_of(const uw_kv8_cache* c, const uw_kv8_seqs* q)
+{
+    Kv8View v;
+    v.k = (uint8_t*)c->k;
+    v.v = (uint8_t*)c->v;
+    v.ks = c->k_scale;
+    v.vs = c->v_scale;
+    v.n_pages = c->n_pages;
+    v.Hkv = c->n_kv_heads;
+    v.P = c->page;
+    v.log2P = log2_page(c->page);
+    v.D = c->head_dim;
+    v.table = q->table;
+    v.width = q->table_width;
+    return v;
+}
+
+static inline TokArg arg_of(const uw_kv8_tokens* t) { return TokArg{t->data, (long)t->seq_stride, (long)t->tok_stride, (long)t->head_stride}; }
+static inline TokSpan span_of(const uw_kv8_seqs* t) { return TokSpan{t->tok_start, t->B, t->T, (long)t->n_tok}; }
+
+#define KV8_DISPATCH(format, dtype, CALL)                                                   \
+    do {                                                                                    \
+        if (format == UW_KV8_INT8) {                                                        \
+            if (dtype == UW_DTYPE_BF16) { CALL(UW_KV8_INT8, bf16_t); } else { CALL(UW_KV8_INT8, float); } \
+        } else {                                                                            \
+            if (dtype == UW_DTYPE_BF16) { CALL(UW_KV8_E4M3, bf16_t); } else { CALL(UW_KV8_E4M3, float); } \
+        }                                                                                   \
+    } while (0)

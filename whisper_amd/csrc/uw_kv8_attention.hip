@@ -1,0 +1,678 @@
+// Attention over the 8-bit paged key/value cache.
+#include "../../include/uw_hip.h"
+#include "uw_kv8.h"
+#include "uw_kernels.h"
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// Attention.  Rows of one kv head are its G query heads of every query token, token-major: row = t * G + g.  A wave works on 64
+// keys at a time and 16 * RT rows, in registers throughout:
+//   S^T = K Q^T    16x16x32 MFMA, A = K codes as bf16 (exact), B = Q; lane (row = lane & 15, g = lane >> 4) gets for tile t the keys
+//                  16 g + 4 t + 0..3, because row slot r of tile t holds key 16 (r >> 2) + 4 t + (r & 3)
+//   O^T = V^T P^T  A = V codes as they lie (16 consecutive keys 16 g .. of one channel), B = P straight from those lanes
+// so neither K nor V nor P passes through LDS.  Scales multiply the scores (K) and the probabilities (V) -- one per 16 keys at
+// least, so one per lane.  Running maximum, sum and output in f32.  f32 queries and probabilities enter as three bf16 planes (24
+// bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.  bf16 queries are exact; their probabilities are
+// rounded to bf16 (2^-9 of each, independently), which is what the output is rounded to anyway.
+struct AttnArgs {
+    Kv8View c;
+    TokSpan ts;
+    TokArg q, o;
+    float* lse;
+    const int32_t* kv_len;
+    float* part;         // [rows][H][n_split][D + 4] partial results (output, maximum, sum) when n_split > 1
+    int H, G, causal;
+    int n_split;         // 1: an item is a row tile of a sequence; else at most so many items share a tile, each with a part of the keys
+    int target, min_chunk;   // n_split > 1: items a head should come to, and the fewest blocks of 64 keys of one
+    int tiles, groups;   // row tiles per sequence (uniform), items of a head
+    int max_blocks;      // blocks that the table can hold, and one more: a longer sequence sees a page that does not exist
+    int lds_rows;        // rows of a tile that can be in use
+    float scale2;        // |scale| * log2(e)
+    unsigned neg;        // sign bit of scale, moved to the queries
+};
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+// 8 codes -> an MFMA operand chunk
+template <int F> __device__ __forceinline__ bf16x8 codes8(unsigned a, unsigned b);
+template <> __device__ __forceinline__ bf16x8 codes8<UW_KV8_E4M3>(unsigned a, unsigned b)
+{
+    union { bf16x2 p[4]; bf16x8 v; } u;
+    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+    return u.v;
+}
+template <> __device__ __forceinline__ bf16x8 codes8<UW_KV8_INT8>(unsigned a, unsigned b)
+{
+    bf16x8 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = (__bf16)(float)(int8_t)(a >> (8 * i));
+        v[4 + i] = (__bf16)(float)(int8_t)(b >> (8 * i));
+    }
+    return v;
+}
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// the planes of 8 f32 values
+template <int NP> __device__ __forceinline__ void planes(const float* x, bf16x8* out)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float rest = x[e];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const __bf16 part = (__bf16)rest;
+            out[n][e] = part;
+            rest -= (float)part;
+        }
+    }
+}
+
+// keeps the first n of 16 bytes
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int n)
+{
+    auto m = [&](int k) { return k <= 0 ? 0u : k >= 4 ? ~0u : (1u << (8 * k)) - 1u; };
+    return make_uint4(v.x & m(n), v.y & m(n - 4), v.z & m(n - 8), v.w & m(n - 12));
+}
+
+// ---- which workgroup does what ------------------------------------------------------------------------------------------
+__device__ __forceinline__ int blocks_of(const AttnArgs& p, int b)
+{
+    const int len = max(0, p.kv_len[b]);
+    return min((len >> 6) + ((len & 63) ? 1 : 0), p.max_blocks);
+}
+__device__ __forceinline__ int tiles_of(const AttnArgs& p, int b, int rows) { return p.ts.tok_start ? (int)(((long)p.ts.count(b) * p.G + rows - 1) / rows) : p.tiles; }
+
+// Keys are cut by what is there, not by what the table could hold: the blocks of all sequences together, over the items wanted.  So
+// unequal lengths give equal items, and a call over one long sequence as many as one over many short ones.
+__device__ __forceinline__ int chunk_of(const AttnArgs& p, int rows)
+{
+    long sum = 0;
+    for (int b = threadIdx.x & 63; b < p.ts.B; b += 64) sum += (long)tiles_of(p, b, rows) * blocks_of(p, b);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    return (int)max((long)p.min_chunk, (sum + p.target - 1) / p.target);
+}
+__device__ __forceinline__ int splits_of(const AttnArgs& p, int b, int chunk) { return max(1, (blocks_of(p, b) + chunk - 1) / chunk); }
+
+// a 16-byte piece of the cache; ONCE: no other workgroup will want it, so it need not stay in L2
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+template <bool ONCE> __device__ __forceinline__ uint4 ld_codes(const void* p)
+{
+    const u32x4 v = ONCE ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// a wave-uniform address, in scalar registers
+__device__ __forceinline__ const uint8_t* in_scalars(const uint8_t* p)
+{
+    const uint64_t u = (uint64_t)p;
+    return (const uint8_t*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)u) | (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32);
+}
+
+// largest of the four lanes that hold a row (lane & 15 alike), without a trip through LDS; a NaN loses
+__device__ __forceinline__ float across_groups_max(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// four channels of a finished row (or of a split's part of it)
+template <typename T, int D>
+__device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first, int kvh, int row, int d, int split, int splits, float M, float L, f32x4 acc)
+{
+    const int t = row / p.G, h = kvh * p.G + row % p.G;
+    const long rg = t_first + t;                        // row of the call
+    if (splits > 1) {
+        float* at = p.part + ((rg * p.H + h) * p.n_split + split) * (D + 4);
+        *(f32x4*)(at + d) = acc;
+        if (d == 0) { at[D] = M; at[D + 1] = L; }
+        return;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    T* out = (T*)p.o.data + (p.ts.tok_start ? rg * p.o.sT : (long)b * p.o.sB + (long)t * p.o.sT) + (long)h * p.o.sH + d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(acc[k] * inv);
+    if (p.lse && d == 0) p.lse[rg * p.H + h] = L == 0.f ? -INFINITY : M * LN2 + logf(L);
+}
+
+// WK waves share the keys of a row tile (their results are joined in LDS), WR row tiles per workgroup
+//
+// RING (WR = 4, pages of 64 tokens or more): the waves work on the same block at the same time, and its codes are brought into LDS once
+// for all of them, STAGES - 1 blocks ahead, by the LDS DMA -- a quarter by each wave, no registers held while they are under way.
+constexpr int STAGES = 4;
+
+template <int F, typename T, int D, int RT, int WK, int WR, bool RING>
+__global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
+{
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
+    constexpr unsigned STAGE_BYTES = 64 * D * 2;
+    static_assert(!RING || (WR == 4 && WK == 1), "a ring is filled and read by four waves of rows");
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % WK, wr = wave / WK;
+    const int rr = lane & 15, g4 = lane >> 4;
+    const Kv8View& c = p.c;
+
+    // which kv head, sequence, rows and part of the keys (heads run fastest: a head's workgroups land on one XCD when their number
+    // is a multiple of 8, and share its L2)
+    int b, tile, split = 0, splits = 1, chunk = 0;
+    const int kvh = blockIdx.x % c.Hkv, item = blockIdx.x / c.Hkv;
+    if (p.n_split > 1) {
+        int j;
+        chunk = chunk_of(p, ROWS * WR);
+        if (!locate(item, p.ts.B, [&](int i) { return tiles_of(p, i, ROWS * WR) * splits_of(p, i, chunk); }, b, j)) return;
+        splits = splits_of(p, b, chunk);
+        tile = j / splits;
+        split = j % splits;
+    } else if (p.ts.tok_start) {
+        if (!locate(item, p.ts.B, [&](int i) { return tiles_of(p, i, ROWS * WR); }, b, tile)) return;
+    } else {
+        b = item / p.tiles;
+        tile = item % p.tiles;
+    }
+    const int n = p.ts.count(b), n_rows = n * p.G;
+    if (p.causal) tile = (n_rows + ROWS * WR - 1) / (ROWS * WR) - 1 - tile;      // rows that see most first
+    const int row0 = (tile * WR + wr) * ROWS;
+    const int len = max(0, p.kv_len[b]);
+    const long t_first = p.ts.first(b);
+
+    // keys each of this lane's rows sees; the fewest and the most of the wave's
+    const int row_end = min(row0 + ROWS, n_rows);
+    auto seen = [&](int row) { return p.causal ? max(0, len - n + 1 + row / p.G) : len; };
+    int lim[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) lim[i] = seen(min(row0 + 16 * i + rr, n_rows - 1));
+    const int lim_min = row0 < n_rows ? seen(row0) : 0, lim_max = row0 < n_rows ? seen(row_end - 1) : 0;
+
+    // Q fragments
+    bf16x8 qf[RT][HALF][2][NP];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int row = row0 + 16 * i + rr;
+        const int t = row / p.G, h = kvh * p.G + row % p.G;
+        const long at = (p.ts.tok_start ? (t_first + t) * p.q.sT : (long)b * p.q.sB + (long)t * p.q.sT) + (long)h * p.q.sH + g4 * 16;
+#pragma unroll
+        for (int hf = 0; hf < HALF; ++hf)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if constexpr (NP == 1) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (row < n_rows) w = *(const uint4*)((const T*)p.q.data + at + hf * 64 + s * 8);
+                    const unsigned flip = p.neg | p.neg >> 16;
+                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+                    qf[i][hf][s][0] = __builtin_bit_cast(bf16x8, w);
+                } else {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = row < n_rows ? to_f32<T>(((const T*)p.q.data)[at + hf * 64 + s * 8 + e]) : 0.f;
+                        x[e] = __uint_as_float(__float_as_uint(x[e]) ^ p.neg);
+                    }
+                    planes<NP>(x, qf[i][hf][s]);
+                }
+            }
+    }
+
+    f32x4 o[RT][D / 16];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[i][d] = f32x4{0, 0, 0, 0};
+    }
+
+    // blocks of 64 keys of this item, dealt to the waves
+    const int blocks = min((lim_max >> 6) + ((lim_max & 63) ? 1 : 0), p.max_blocks);
+    const int blk0 = split * chunk, blk1 = splits > 1 ? min(blocks, blk0 + chunk) : blocks;
+    const long page_bytes = (long)c.P * D;
+    const int k_group = 16 * (rr >> 2), k_in = rr & 3;     // 16-key group and place in it of this lane's K rows
+    int blk = blk0 + wk;
+
+    // 64 pages from the one of block `blk` on, one to a lane: id and scales, so that a step asks memory for nothing but codes
+    int win = 0, w_id = -1;
+    float w_ks = 0.f, w_vs = 0.f;
+    auto window = [&](int from) {
+        win = (from << 6) >> c.log2P;
+        w_id = kv8_page(c, b, (long)win + lane);
+        w_ks = w_vs = __uint_as_float(0x7fc00000u);
+        if (w_id >= 0) {
+            w_ks = c.ks[(long)w_id * c.Hkv + kvh] * p.scale2;
+            w_vs = c.vs[(long)w_id * c.Hkv + kvh];
+        }
+    };
+    // whether the pages of block x are in it
+    auto in_window = [&](int x) { return (((x << 6) + 48) >> c.log2P) - win < 64; };
+    // lane of the window that holds key j's page
+    auto at_key = [&](int j) { return (j >> c.log2P) - win; };
+
+    uint4 kf[4][HALF], vf[D / 16];
+    auto load_k = [&](int x) {
+        const int j = (x << 6) + k_group, id = max(0, __shfl(w_id, at_key(j), 64));
+        const uint8_t* kp = c.k + ((long)id * c.Hkv + kvh) * page_bytes + ((j & (c.P - 1)) + k_in) * D + g4 * 16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = ld_codes<(RT == 1)>(kp + t * 4 * D + hf * 64);
+    };
+    auto load_v = [&](int x) {
+        const int j = (x << 6) + 16 * g4, id = max(0, __shfl(w_id, at_key(j), 64));
+        const uint8_t* vp = c.v + ((long)id * c.Hkv + kvh) * page_bytes + rr * c.P + (j & (c.P - 1));
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(RT == 1)>(vp + d * 16 * c.P);
+    };
+    // RING: a wave asks for its share of a block, straight into LDS in the order the lanes hold it; `stage` of block x is x mod STAGES
+    uint4* const ring = (uint4*)lds;
+    const unsigned ring_at = RING ? lds_addr_of(lds) : 0;
+    auto request = [&](int x) {
+        const int id = max(0, __builtin_amdgcn_readlane(w_id, at_key(x << 6)));
+        const int in_page = (x << 6) & (c.P - 1);
+        const long at = ((long)id * c.Hkv + kvh) * page_bytes;
+        const uint8_t* kp = in_scalars(c.k + at + in_page * D);
+        const uint8_t* vp = in_scalars(c.v + at + in_page);
+        const unsigned to = ring_at + (unsigned)(x % STAGES) * STAGE_BYTES;
+#pragma unroll
+        for (int hf = 0; hf < HALF; ++hf) {
+            glds16_sv(kp, (unsigned)((k_group + k_in + 4 * wr) * D + hf * 64 + g4 * 16), to + (wr * HALF + hf) * 1024);
+            glds16_sv(vp, (unsigned)(((hf * 4 + wr) * 16 + rr) * c.P + g4 * 16), to + (4 * HALF + hf * 4 + wr) * 1024);
+        }
+    };
+    if (!RING && blk < blk1) {
+        window(blk);
+        load_k(blk);
+        load_v(blk);
+    }
+    // one step; MASK: some row does not see all 64 keys
+    auto step = [&](auto masked) __attribute__((always_inline)) {
+        constexpr bool mask = decltype(masked)::value;
+        const int j0 = blk << 6, jv = j0 + 16 * g4;
+        const bool more = !RING && blk + WK < blk1;
+        const float kscale = __shfl(w_ks, at_key(jv), 64), vs = __shfl(w_vs, at_key(jv), 64);
+        if (more && !in_window(blk + WK)) window(blk + WK);
+        if constexpr (RING) {
+            const uint4* from = ring + (blk % STAGES) * (STAGE_BYTES / 16) + lane;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = from[(t * HALF + hf) * 64];
+        }
+
+        f32x4 st[RT][4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) st[i][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int hf = 0; hf < HALF; ++hf) {
+                const bf16x8 a0 = codes8<F>(kf[t][hf].x, kf[t][hf].y), a1 = codes8<F>(kf[t][hf].z, kf[t][hf].w);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int pl = NP - 1; pl >= 0; --pl) {
+                        st[i][t] = mfma(a0, qf[i][hf][0][pl], st[i][t]);
+                        st[i][t] = mfma(a1, qf[i][hf][1][pl], st[i][t]);
+                    }
+            }
+        if constexpr (!RING) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_k(blk + WK);          // in flight under the softmax and P.V
+            __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // a block of zeros (scale 0) has codes of zero: any scale does.  The V scale rides in the exponent: p' = p * vs costs nothing per
+        // element, the sum is divided by it once per block (the rounding of log2(vs) adds |log2 vs| 2^-24 to an element)
+        const float vsc = vs == 0.f ? 1.f : vs, lv = __builtin_amdgcn_logf(vsc), iv = __builtin_amdgcn_rcpf(vsc);
+        bf16x8 pf[RT][2][NP];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int left = lim[i] - jv;          // keys of this lane's 16 that the row sees
+            if constexpr (mask) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (4 * t + e >= left) st[i][t][e] = -INFINITY;
+            }
+            float x[16], sum;
+            auto weigh = [&](float base) {
+                const float nb = lv - base;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] = __builtin_amdgcn_exp2f(fmaf(st[i][k >> 2][k & 3], kscale, nb));
+                if constexpr (mask) {                            // a scale behind the end may be NaN
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (k >= left) x[k] = 0.f;
+                }
+                sum = x[0];
+#pragma unroll
+                for (int k = 1; k < 16; ++k) sum += x[k];
+            };
+            // The reference that scores are taken against need not be the largest so far, only near it: it moves when a lane's 16
+            // weights add up to more than 2^10 (at the first block it is -inf, the sum +inf), so that most blocks look for no maximum
+            // and rescale nothing.  Weights stay below 2^10, sums and outputs in f32; bf16 keeps its 8 bits at any size.
+            bool follow = true;
+            if constexpr (!mask) {
+                weigh(m[i]);
+                follow = __any(sum * iv > 1024.f);
+            }
+            if (follow) {
+                float mx = fmaxf(st[i][0][0], st[i][0][1]);
+#pragma unroll
+                for (int k = 2; k < 16; k += 2) mx = fmaxf(fmaxf(mx, st[i][k >> 2][k & 3]), st[i][k >> 2][(k & 3) + 1]);
+                mx *= kscale;
+                if (mask && left <= 0) mx = -INFINITY;      // nothing of these 16 keys is seen, and the scale may be any leftover
+                mx = across_groups_max(mx);
+                const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
+                l[i] *= alpha;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) o[i][d] *= alpha;
+                m[i] = mn;
+                weigh(base);
+            }
+            // (a poisoned scale of a block that is seen shows in the sum)
+            if (!mask || left > 0) l[i] = fmaf(sum, iv, l[i]);
+            planes<NP>(x, pf[i][0]);
+            planes<NP>(x + 8, pf[i][1]);
+        }
+        if constexpr (RING) {
+            const uint4* from = ring + (blk % STAGES) * (STAGE_BYTES / 16) + 4 * HALF * 64 + lane;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) vf[d] = from[d * 64];
+        }
+        if constexpr (mask) {      // leftovers behind the sequence's end may hold NaN, which a probability of 0 does not silence
+            const int keep = max(0, min(16, len - jv));
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) vf[d] = first_bytes(vf[d], keep);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            const bf16x8 a0 = codes8<F>(vf[d].x, vf[d].y), a1 = codes8<F>(vf[d].z, vf[d].w);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int pl = NP - 1; pl >= 0; --pl) {
+                    o[i][d] = mfma(a0, pf[i][0][pl], o[i][d]);
+                    o[i][d] = mfma(a1, pf[i][1][pl], o[i][d]);
+                }
+        }
+        if constexpr (!RING) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_v(blk + WK);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto steps = [&](int end) {
+        for (; blk < end; blk += WK) {
+            if (lim_min - (blk << 6) < 64) step(std::true_type{});
+            else step(std::false_type{});
+        }
+    };
+    if constexpr (!RING) {
+        steps(blk1);
+    } else {
+        // the waves go through the blocks together, as far as the one that sees most; requests run STAGES - 1 blocks ahead
+        const int all_end = min((tile * WR + WR) * ROWS, n_rows);
+        const int most = all_end > 0 ? seen(all_end - 1) : 0, end = min((most >> 6) + ((most & 63) ? 1 : 0), p.max_blocks);
+        if (end > 0) window(0);
+        for (int x = 0; x < min(STAGES - 1, end); ++x) request(x);
+        for (blk = 0; blk < end;) {
+            // this block's pieces of this wave have landed when at most the later blocks' are under way; then everybody's have.  Whoever
+            // passes the barrier is done with block blk - 1, whose stage the next request takes.
+            if (blk + STAGES - 1 < end) __builtin_amdgcn_s_waitcnt(0x0F70 | ((STAGES - 2) * 2 * HALF));
+            else __builtin_amdgcn_s_waitcnt(0x0F70);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (blk + STAGES - 1 < end) {
+                if (!in_window(blk + STAGES - 1)) window(blk);
+                request(blk + STAGES - 1);
+            }
+            if (blk < blk1) steps(blk + 1);
+            else ++blk;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        l[i] += __shfl_xor(l[i], 16, 64);
+        l[i] += __shfl_xor(l[i], 32, 64);
+    }
+
+    // join the waves that shared the keys
+    if constexpr (WK > 1) {
+        const int R = p.lds_rows;
+        float* sm = lds + (long)wr * WK * R * (D + 2);                    // [WK][R] m, [WK][R] l, [WK][R][D]
+        float* sl = sm + WK * R;
+        float* so = sl + WK * R;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int r = 16 * i + rr;
+            if (r >= R) continue;
+            if (g4 == 0) { sm[wk * R + r] = m[i]; sl[wk * R + r] = l[i]; }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                float* at = so + ((long)wk * R + r) * D + d * 16 + g4 * 4;
+                at[0] = o[i][d][0]; at[1] = o[i][d][1]; at[2] = o[i][d][2]; at[3] = o[i][d][3];
+            }
+        }
+        __syncthreads();
+        for (int e = (wk * 64 + lane) * 4; e < (row_end - row0) * D; e += 64 * WK * 4) {
+            const int r = e / D, d = e % D;
+            float M = -INFINITY, L = 0.f;
+            f32x4 acc = {0, 0, 0, 0};
+            for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[w * R + r]);
+            for (int w = 0; w < WK; ++w) {
+                // a wave without a finite score has a sum of 0, or NaN where it met a NaN
+                const float mw = sm[w * R + r], f = mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - M);
+                L += sl[w * R + r] * f;
+                const float* x = so + ((long)w * R + r) * D + d;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] += x[k] * f;
+            }
+            store_row<T, D>(p, b, t_first, kvh, row0 + r, d, split, splits, M, L, acc);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int row = row0 + 16 * i + rr;
+            if (row < n_rows)
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) store_row<T, D>(p, b, t_first, kvh, row, d * 16 + g4 * 4, split, splits, m[i], l[i], o[i][d]);
+        }
+    }
+}
+
+// joins the parts of a row whose keys were cut: a wave per (token, head)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p, int tile_rows)
+{
+    const int lane = threadIdx.x & 63;
+    const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6), row = w / p.H;
+    const int h = (int)(w % p.H);
+    if (row >= p.ts.N) return;
+    int b = 0;
+    long oat = row * p.o.sT;
+    if (p.ts.tok_start) {
+        // the last sequence that begins at or before the row (those behind it are empty or later)
+        int n = 0;
+        for (int i = lane; i < p.ts.B; i += 64) n += p.ts.tok_start[i] <= row ? 1 : 0;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+        b = n - 1;
+        if (b < 0 || row >= p.ts.tok_start[b] + (long)p.ts.count(b)) return;
+    } else {
+        b = (int)(row / p.ts.T);
+        oat = (long)b * p.o.sB + row % p.ts.T * p.o.sT;
+    }
+    const int splits = splits_of(p, b, chunk_of(p, tile_rows));
+    if (splits == 1) return;                         // its workgroup wrote the result
+    const float* part = p.part + w * p.n_split * (D + 4);
+    float M = -INFINITY, L = 0.f, acc[D / 64] = {};
+    for (int s = lane; s < splits; s += 64) M = fmaxf(M, part[s * (D + 4) + D]);
+    M = wave_max(M);
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float* x = part + s * (D + 4);
+        const float ms = x[D], ls = x[D + 1];
+        const float f = ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms - M);
+        L += ls * f;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) acc[k] += x[k * 64 + lane] * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) ((T*)p.o.data)[oat + (long)h * p.o.sH + k * 64 + lane] = from_f32<T>(acc[k] * inv);
+    if (p.lse && lane == 0) p.lse[row * p.H + h] = L == 0.f ? -INFINITY : M * LN2 + logf(L);
+}
+
+// ---- host side --------------------------------------------------------------------------------------
+int check_attention(const char* fn, const uw_kv8_attention_args* a)
+{
+    UW_REQUIRE(a, "%s: null arguments", fn);
+    RUN(check_cache(fn, &a->cache));
+    RUN(check_seqs(fn, &a->seqs));
+    RUN(check_tokens(fn, "q", &a->q, &a->seqs));
+    RUN(check_tokens(fn, "o", &a->o, &a->seqs));
+    UW_REQUIRE(a->n_heads > 0 && a->n_heads % a->cache.n_kv_heads == 0, "%s: %d query heads over %d kv heads", fn, a->n_heads, a->cache.n_kv_heads);
+    return UW_OK;
+}
+
+// row tiles of 16 that a wave's registers hold: f32 keeps three planes of its queries, which 128 channels leave room for once
+constexpr int max_row_tiles(size_t elem, int D) { return elem == 4 && D == 128 ? 1 : 2; }
+
+struct AttnPlan {
+    int rt, wk, wr;      // row tiles of 16 per wave, waves sharing keys, waves side by side on rows
+    bool ring;
+    int n_split, target, min_chunk, tiles, max_blocks, lds_rows;
+    long groups, ws_bytes;
+};
+
+// How a call is cut.
+//  - up to 16 rows of a kv head: one row tile, the waves share the keys
+//  - more: tiles of 128 rows, 32 to a wave, if there are enough of them to fill the chip; else tiles of 32 rows whose four waves share
+//    the keys -- four times the workgroups for the same rows
+//  - long sequences are cut further where the waves share the keys, into items of equal size (chunk_of), joined by a second launch
+AttnPlan plan_attention(const uw_kv8_attention_args* a)
+{
+    AttnPlan p;
+    const uw_kv8_cache* c = &a->cache;
+    const int G = a->n_heads / c->n_kv_heads, B = a->seqs.B, T = a->seqs.tok_start ? 0 : a->seqs.T;
+    const int64_t n_tok = a->seqs.n_tok;
+    const long rows = T > 0 ? (long)T * G : (long)ceil_div(n_tok, B) * G;     // per sequence; packed: on average
+    p.max_blocks = (int)std::min((long)ceil_div((long)a->seqs.table_width * c->page, 64) + 1, (1l << 25) - 1);
+    p.rt = rows <= 16 ? 1 : max_row_tiles(a->seqs.dtype == UW_DTYPE_F32 ? 4 : 2, c->head_dim);
+    p.wk = 4;
+    p.wr = 1;
+    if (rows > 32 && (long)ceil_div(rows, 64 * p.rt) * B * c->n_kv_heads >= 384) {
+        p.wk = 1;
+        p.wr = 4;
+    }
+    p.ring = p.wr == 4 && c->page >= 64;
+    const int per = 16 * p.rt * p.wr;
+    p.tiles = T > 0 ? ceil_div(rows, per) : 0;
+    p.groups = T > 0 ? (long)B * p.tiles : n_tok * G / per + std::min((long)B, (long)n_tok);
+    const long alone = p.groups * c->n_kv_heads;             // workgroups without a cut
+    p.n_split = 1;
+    p.target = p.min_chunk = 0;
+    if (p.wk == 4 && p.max_blocks > 33 && !(alone >= 512 && p.max_blocks <= 65)) {
+        p.min_chunk = 8;
+        // a tile's last item is a short one: they are counted in, so that all items find a place at once
+        const long items = ceil_div(512, c->n_kv_heads);
+        p.target = (int)std::max(std::max(items - p.groups, items / 2), 1l);
+        p.n_split = std::min(p.target, ceil_div(p.max_blocks, p.min_chunk));
+        if (p.n_split > 1) p.groups += p.target;
+    }
+    p.lds_rows = T > 0 ? (int)std::min((long)16 * p.rt, rows) : 16 * p.rt;
+    if (p.wk == 4 && p.rt == 1 && p.n_split == 1 && alone <= 256) p.wk = 8;       // few workgroups: more waves in each
+    p.ws_bytes = p.n_split > 1 ? n_tok * a->n_heads * (int64_t)p.n_split * (c->head_dim + 4) * 4 : 0;
+    return p;
+}
+
+template <int F, typename T, int D, int RT, int WK, int WR, bool RING> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+{
+    const size_t lds = RING ? (size_t)STAGES * 64 * D * 2 : WK > 1 ? (size_t)WR * WK * p.lds_rows * (D + 2) * 4 : 0;
+    if (lds > 64 * 1024) {
+        static PerDeviceFlag flag;
+        if (flag.pending()) {
+            UW_HIP_CHECK(hipFuncSetAttribute((const void*)kv8_attention_kernel<F, T, D, RT, WK, WR, RING>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            flag.mark();
+        }
+    }
+    hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR, RING>), dim3((unsigned)(p.groups * a.c.Hkv)), dim3(64 * WK * WR), lds, s, a);
+    UW_LAUNCH_CHECK();
+    return UW_OK;
+}
+
+template <int F, typename T, int D> int launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+{
+    constexpr int RT = max_row_tiles(sizeof(T), D);
+    if (p.ring) return launch_attention_as<F, T, D, RT, 1, 4, true>(a, p, s);
+    if (p.wr == 4) return launch_attention_as<F, T, D, RT, 1, 4, false>(a, p, s);
+    if (p.wk == 8) return launch_attention_as<F, T, D, 1, 8, 1, false>(a, p, s);
+    if (p.rt == 1) RUN((launch_attention_as<F, T, D, 1, 4, 1, false>(a, p, s)));
+    if constexpr (RT > 1) {
+        if (p.rt == RT) RUN((launch_attention_as<F, T, D, RT, 4, 1, false>(a, p, s)));
+    }
+    if (p.n_split == 1) return UW_OK;
+    hipLaunchKernelGGL((kv8_join_kernel<T, D>), dim3(ceil_div(a.ts.N * a.H, 4)), dim3(256), 0, s, a, 16 * p.rt);
+    UW_LAUNCH_CHECK();
+    return UW_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_attention_args* a)
+{
+    if (check_attention("uw_kv8_attention_workspace_bytes", a)) return -1;
+    return a->seqs.n_tok ? plan_attention(a).ws_bytes : 0;
+}
+
+int uw_kv8_attention(const uw_kv8_attention_args* a, void* stream)
+{
+    RUN(check_attention("uw_kv8_attention", a));
+    const uw_kv8_seqs& q = a->seqs;
+    if (q.n_tok == 0) return UW_OK;
+    const AttnPlan pl = plan_attention(a);
+    UW_REQUIRE(pl.ws_bytes == 0 || (a->ws && ((uintptr_t)a->ws & 15) == 0 && a->ws_bytes >= pl.ws_bytes),
+               "uw_kv8_attention: workspace missing, misaligned or smaller than %lld bytes", (long long)pl.ws_bytes);
+    UW_REQUIRE(pl.groups * a->cache.n_kv_heads < (1 << 22) && q.n_tok * a->n_heads <= 0x7fffffff, "uw_kv8_attention: too many rows");
+    AttnArgs x;
+    x.c = view_of(&a->cache, &q);
+    x.ts = span_of(&q);
+    x.q = arg_of(&a->q);
+    x.o = arg_of(&a->o);
+    x.lse = a->lse;
+    x.kv_len = q.len;
+    x.part = (float*)a->ws;
+    x.H = a->n_heads;
+    x.G = a->n_heads / a->cache.n_kv_heads;
+    x.causal = a->causal;
+    x.n_split = pl.n_split;
+    x.target = pl.target;
+    x.min_chunk = pl.min_chunk;
+    x.max_blocks = pl.max_blocks;
+    x.tiles = pl.tiles;
+    x.groups = (int)pl.groups;
+    x.lds_rows = pl.lds_rows;
+    x.scale2 = fabsf(a->scale) * LOG2E;
+    x.neg = a->scale < 0.f ? 0x80000000u : 0u;
+#define CALL(F, T) RUN((a->cache.head_dim == 64 ? launch_attention<F, T, 64>(x, pl, (hipStream_t)stream) : launch_attention<F, T, 128>(x, pl, (hipStream_t)stream)))
+    KV8_DISPATCH(a->cache.format, q.dtype, CALL);
+#undef CALL
+    return UW_OK;
+}
+
+}  // extern "C"
