@@ -22,14 +22,14 @@ struct Kv8View {
 struct TokSpan {
     const int32_t* tok_start;   // null: uniform
     int B, T;                   // T: tokens per sequence (uniform only)
-    long N;                     // rows altogether
+    int N;                      // rows altogether
     __device__ __forceinline__ long first(int b) const { return tok_start ? (long)tok_start[b] : (long)b * T; }
     // tokens of sequence b; a malformed tok_start gives 0 rather than rows outside [0, N)
     __device__ __forceinline__ int count(int b) const
     {
         if (!tok_start) return T;
-        const long s = tok_start[b], e = tok_start[b + 1];
-        return (s < 0 || e > N || e < s) ? 0 : (int)(e - s);
+        const int s = tok_start[b], e = tok_start[b + 1];
+        return (s < 0 || e > N || e < s) ? 0 : e - s;
     }
 };
 
@@ -42,10 +42,6 @@ __device__ __forceinline__ int kv8_page(const Kv8View& c, int b, long blk)
 }
 
 // ---- code <-> value ---------------------------------------------------------------------------------
-template <int F> __device__ __forceinline__ float kv8_decode(uint8_t c);
-template <> __device__ __forceinline__ float kv8_decode<UW_KV8_INT8>(uint8_t c) { return (float)(int8_t)c; }
-template <> __device__ __forceinline__ float kv8_decode<UW_KV8_E4M3>(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
-
 // Codes of four values under the reciprocal scale r.  int8: the 48-bit product is taken in f64, so that it is rounded once and the
 // code is the definition's whatever the order of evaluation; e4m3: r is a power of two, the f32 product is exact where it matters.
 template <int F> __device__ __forceinline__ unsigned kv8_encode4(const float* x, float r);
@@ -65,6 +61,29 @@ template <> __device__ __forceinline__ unsigned kv8_encode4<UW_KV8_E4M3>(const f
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = fminf(fmaxf(x[i] * r, -448.f), 448.f);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+}
+
+template <int F> __device__ __forceinline__ void kv8_decode4(unsigned w, float* x);
+template <> __device__ __forceinline__ void kv8_decode4<UW_KV8_INT8>(unsigned w, float* x)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+}
+template <> __device__ __forceinline__ void kv8_decode4<UW_KV8_E4M3>(unsigned w, float* x)
+{
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+}
+
+// byte j of word i <-> byte i of word j
+__device__ __forceinline__ void transpose4(unsigned* w)
+{
+    const unsigned a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+    const unsigned c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302);
 }
 
 // smallest e with 2^e >= v, v a positive normal number
@@ -94,39 +113,53 @@ struct TokArg {
     long sB, sT, sH;
 };
 
+// sums of lanes 0 .. own, in the vector ALU (row shifts, then the rows' totals handed on)
+__device__ __forceinline__ int wave_scan(int x)
+{
+#define KV8_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, true)
+    KV8_SCAN_STEP(0x111, 0xf);
+    KV8_SCAN_STEP(0x112, 0xf);
+    KV8_SCAN_STEP(0x114, 0xf);
+    KV8_SCAN_STEP(0x118, 0xf);
+    KV8_SCAN_STEP(0x142, 0xa);
+    KV8_SCAN_STEP(0x143, 0xc);
+#undef KV8_SCAN_STEP
+    return x;
+}
+
 // The idx-th (sequence, part) pair of a call, parts counted over the sequences in order; false past the last one.  cnt(b) = parts of
 // sequence b.  Every wave works it out for itself: 256 sequences per step, four to a lane so that their lengths are asked for at
-// once, and one shuffle scan.
+// once, and one scan.
 template <typename CNT> __device__ __forceinline__ bool locate(int idx, int B, CNT cnt, int& b_out, int& j_out)
 {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int b0 = 0; b0 < B; b0 += 256) {
-        const int first = b0 + lane * 4;
         int n[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n[i] = first + i < B ? cnt(first + i) : 0;
-        const int own = (n[0] + n[1]) + (n[2] + n[3]);
-        int incl = own;
+        for (int i = 0; i < 4; ++i) n[i] = 0;
+        const int first = b0 + lane * 4;
+        if (first < B) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += up;
+            for (int i = 0; i < 4; ++i) n[i] = cnt(min(first + i, B - 1));
+#pragma unroll
+            for (int i = 1; i < 4; ++i) n[i] = first + i < B ? n[i] : 0;
         }
+        const int own = (n[0] + n[1]) + (n[2] + n[3]), incl = wave_scan(own);
         const unsigned long long over = __ballot(base + incl > idx);
         if (over) {
             const int w = __ffsll((long long)over) - 1;
-            int j = idx - base - __shfl(incl - own, w, 64), b = b0 + w * 4;
+            int j = idx - base - __builtin_amdgcn_readlane(incl - own, w), b = b0 + w * 4;
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
-                const int c = __shfl(n[i], w, 64);
+                const int c = __builtin_amdgcn_readlane(n[i], w);
                 if (b == b0 + w * 4 + i && j >= c) { j -= c; ++b; }
             }
-            b_out = __builtin_amdgcn_readfirstlane(b);
-            j_out = __builtin_amdgcn_readfirstlane(j);
+            b_out = b;
+            j_out = j;
             return true;
         }
-        base += __shfl(incl, 63, 64);
+        base += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
 }
@@ -191,7 +224,7 @@ static inline Kv8View view_of(const uw_kv8_cache* c, const uw_kv8_seqs* q)
 }
 
 static inline TokArg arg_of(const uw_kv8_tokens* t) { return TokArg{t->data, (long)t->seq_stride, (long)t->tok_stride, (long)t->head_stride}; }
-static inline TokSpan span_of(const uw_kv8_seqs* t) { return TokSpan{t->tok_start, t->B, t->T, (long)t->n_tok}; }
+static inline TokSpan span_of(const uw_kv8_seqs* t) { return TokSpan{t->tok_start, t->B, t->T, (int)t->n_tok}; }
 
 #define KV8_DISPATCH(format, dtype, CALL)                                                   \
     do {                                                                                    \
