@@ -21,7 +21,7 @@ namespace {
 constexpr int CHUNK = 4096, PER = 16;      // scores per workgroup and per thread
 
 struct ChunkStat { double z; float mx; int arg; };         // sum of exp((x - mx) / T), maximum, its lowest index (-1: a NaN, greedy only)
-struct Chosen { double zp, zq; float mp, mq; int acc, mode; };   // the rows drawn from; mode 0: p alone, 1: p - q, 2: p without the drafted token
+struct Chosen { double rp, rq; float mp, mq; int acc, mode; };   // the rows drawn from (1 / sum, maximum); mode 0: p alone, 1: p - q, 2: p without the drafted token
 
 struct VerifyParams {
     const void *target, *draft;
@@ -150,77 +150,80 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p)
     }
 }
 
-// maximum and sum of a whole row from its chunks; one wave, the same in all lanes and -- the order being fixed -- in all workgroups
+// maximum and sum of a whole row from its chunks, by 16 lanes, the same in all of them and -- the order being fixed -- in all workgroups
 __device__ __forceinline__ void join_row(const ChunkStat* st, int chunks, double inv_t, float& m, double& z)
 {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 15;
     m = -INFINITY;
-    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, st[c].mx);
-    m = wave_max(m);
+    for (int c = lane; c < chunks; c += 16) m = fmaxf(m, st[c].mx);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     z = 0;
-    for (int c = lane; c < chunks; c += 64) {
+    for (int c = lane; c < chunks; c += 16) {
         const ChunkStat s = st[c];
         z += s.mx == -INFINITY ? s.z : s.z * exp_neg(((double)s.mx - (double)m) * inv_t);    // (z of a chunk of -inf is 0, or NaN)
     }
-    z = wave_sum_d(z);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+}
+
+// r: 1 / sum of the row's exponentials
+__device__ __forceinline__ double probability(const VerifyParams& p, float x, float m, double r)
+{
+    return p.probs ? (double)x : exp_neg(((double)x - (double)m) * p.inv_t) * r;
 }
 
 // (2) grid (chunks, B)
 template <typename T>
 __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
 {
-    __shared__ int s_ok[4];
-    __shared__ double s_z[4], s_r[4];
-    __shared__ float s_m[2];
+    __shared__ double s_r[16], s_p[16], s_z[4], s_w[4];        // of a batch of rows: 1 / sum, probability of the drafted token
+    __shared__ float s_m[16], s_u[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x % p.chunks, b = blockIdx.x / p.chunks;
     const int n = p.n_of(b), V = p.V;
     const T* tb = (const T*)p.target + (long)b * p.t_sB;
     const T* db = p.draft ? (const T*)p.draft + (long)b * p.d_sB : nullptr;
     const int32_t* d = p.drafted + (long)b * p.N;
-    const ChunkStat* ts = p.t_stat + (long)b * (p.N + 1) * p.chunks;
-    const ChunkStat* ds = p.d_stat + (long)b * p.N * p.chunks;
-    const auto probability = [&](float x, float m, double z) { return p.probs ? (double)x : exp_neg(((double)x - (double)m) * p.inv_t) / z; };
+    const float* u = p.u + (long)b * (p.N + 1);
 
-    // how many tokens stand: four at a time, a wave each
-    int acc = 0;
-    for (int i0 = 0; i0 < n; i0 += 4) {
-        const int i = i0 + wave;
-        bool ok = false;
-        if (i < n && d[i] >= 0 && d[i] < V) {
+    // How many tokens stand.  Eight positions at a time, 16 lanes to a row: even slots the target's rows, odd ones the draft's, so that
+    // all their statistics are on their way at once.
+    int acc;
+    for (int i0 = 0;; i0 += 8) {
+        const int slot = tid >> 4, i = i0 + (slot >> 1);
+        const bool is_draft = slot & 1;
+        if (i <= n && (!is_draft || (db && i < n))) {
+            const int di = i < n ? d[i] : -1;
+            const bool token = di >= 0 && di < V;
+            const float x = !token ? 0.f : is_draft ? to_f32<T>(db[(long)i * p.d_sN + di]) : to_f32<T>(tb[(long)i * p.t_sN + di]);
             float m = 0;
             double z = 1;
-            if (!p.probs) join_row(ts + (long)i * p.chunks, p.chunks, p.inv_t, m, z);
-            const double pd = probability(to_f32<T>(tb[(long)i * p.t_sN + d[i]]), m, z);
-            double qd = 1.0;
-            if (db) {
-                if (!p.probs) join_row(ds + (long)i * p.chunks, p.chunks, p.inv_t, m, z);
-                qd = probability(to_f32<T>(db[(long)i * p.d_sN + d[i]]), m, z);
+            if (!p.probs) {
+                if (is_draft) join_row(p.d_stat + ((long)b * p.N + i) * p.chunks, p.chunks, p.inv_t, m, z);
+                else join_row(p.t_stat + ((long)b * (p.N + 1) + i) * p.chunks, p.chunks, p.inv_t, m, z);
             }
-            ok = (double)p.u[(long)b * (p.N + 1) + i] * qd < pd;
+            const double r = 1.0 / z;
+            if ((tid & 15) == 0) {
+                if (!is_draft) s_u[slot >> 1] = i < n ? u[i] : 0.f;
+                s_m[slot] = m;
+                s_r[slot] = r;
+                s_p[slot] = !token ? 0.0 : probability(p, x, m, r);       // an id outside the vocabulary is never accepted
+            }
         }
-        if (lane == 0) s_ok[wave] = ok;
         __syncthreads();
-        const int run = !s_ok[0] ? 0 : !s_ok[1] ? 1 : !s_ok[2] ? 2 : !s_ok[3] ? 3 : 4;
-        __syncthreads();
+        int run = 0;
+        while (run < 8 && i0 + run < n && (double)s_u[run] * (db ? s_p[2 * run + 1] : 1.0) < s_p[2 * run]) ++run;
         acc = i0 + run;
-        if (run < 4) break;
+        if (run < 8) break;
+        __syncthreads();
     }
-    acc = min(acc, n);
 
     // the rows that the next token is drawn from
     const T* row = tb + (long)acc * p.t_sN;
     const T* qrow = (db && acc < n) ? db + (long)acc * p.d_sN : nullptr;
-    const int point = (!db && acc < n && d[acc] >= 0 && d[acc] < V) ? d[acc] : -1;
-    if (!p.probs && (wave == 0 || (wave == 1 && qrow))) {
-        float m;
-        double z;
-        join_row(wave ? ds + (long)acc * p.chunks : ts + (long)acc * p.chunks, p.chunks, p.inv_t, m, z);
-        if (lane == 0) { s_m[wave] = m; s_z[wave] = z; }
-    }
-    __syncthreads();
-    const float mp = p.probs ? 0.f : s_m[0], mq = (p.probs || !qrow) ? 0.f : s_m[1];
-    const double zp = p.probs ? 1.0 : s_z[0], zq = (p.probs || !qrow) ? 1.0 : s_z[1];
-    __syncthreads();
+    const int point = (!db && acc < n && d[acc] >= 0 && d[acc] < V) ? d[acc] : -1, at_slot = (acc & 7) * 2;
+    const float mp = s_m[at_slot], mq = qrow ? s_m[at_slot + 1] : 0.f;
+    const double rp = s_r[at_slot], rq = qrow ? s_r[at_slot + 1] : 1.0;
 
     float x[PER], y[PER];
     const int j0 = c * CHUNK;
@@ -230,10 +233,10 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
     double sp = 0, sr = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-        const double w = probability(x[k], mp, zp);
+        const double w = probability(p, x[k], mp, rp);
         sp += w;
         if (qrow) {
-            const double r = w - probability(y[k], mq, zq);
+            const double r = w - probability(p, y[k], mq, rq);
             sr += r != r ? r : fmax(r, 0.0);
         } else if (score_index<T>(j0, k) != point) {
             sr += w;
@@ -241,13 +244,13 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
     }
     sp = wave_sum_d(sp);
     sr = wave_sum_d(sr);
-    if (lane == 0) { s_z[wave] = sp; s_r[wave] = sr; }
+    if (lane == 0) { s_z[wave] = sp; s_w[wave] = sr; }
     __syncthreads();
     if (tid == 0) {
         double* at = p.mass + ((long)b * p.chunks + c) * 2;
-        at[0] = (s_r[0] + s_r[1]) + (s_r[2] + s_r[3]);
+        at[0] = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
         at[1] = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
-        if (c == 0) p.chosen[b] = Chosen{zp, zq, mp, mq, acc, qrow ? 1 : point >= 0 ? 2 : 0};
+        if (c == 0) p.chosen[b] = Chosen{rp, rq, mp, mq, acc, qrow ? 1 : point >= 0 ? 2 : 0};
     }
 }
 
@@ -269,33 +272,37 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
     const Chosen ch = p.chosen[b];
     const double* mass = p.mass + (long)b * p.chunks * 2;
-    // totals of the residual and of p, over the chunks in order
-    double tot[2] = {0, 0};
-    for (int c0 = 0; c0 < p.chunks; c0 += 128) {
-        __syncthreads();
-        if (c0 + (tid >> 1) < p.chunks) s_c[tid] = mass[(long)c0 * 2 + tid];
-        __syncthreads();
-        for (int c = 0; c < min(128, p.chunks - c0); ++c) { tot[0] += s_c[2 * c]; tot[1] += s_c[2 * c + 1]; }
-    }
+    // totals of the residual and of p: a thread a chunk, added up wave by wave in a fixed order
+    double own[2] = {0, 0};
+    for (int c = tid; c < p.chunks; c += 256) { own[0] += mass[2 * c]; own[1] += mass[2 * c + 1]; }
+    own[0] = wave_sum_d(own[0]);
+    own[1] = wave_sum_d(own[1]);
+    if (lane == 0) { s_c[wave] = own[0]; s_c[4 + wave] = own[1]; }
+    __syncthreads();
+    const double tot[2] = {(s_c[0] + s_c[1]) + (s_c[2] + s_c[3]), (s_c[4] + s_c[5]) + (s_c[6] + s_c[7])};
     // an empty residual (probabilities that do not add up alike) leaves the row itself
     const int which = (ch.mode == 0 || tot[0] == 0.0) ? 1 : 0;
     const double total = tot[which];
     if (!(total > 0.0 && total < INFINITY)) { write_tokens(p, b, ch.acc, -1); return; }
     const double r = (double)p.u[(long)b * (p.N + 1) + p.N] * total;
-    if (tid == 0) {
-        // the first chunk whose cumulative weight exceeds r; if rounding leaves none, the last one with weight
-        double cum = 0, before = 0;
+    // the first chunk whose cumulative weight exceeds r; if rounding leaves none, the last one with weight
+    if (wave == 0) {
+        double cum = 0, before = 0, last_before = 0;
         int at = -1, last = 0;
-        double last_before = 0;
-        for (int c = 0; c < p.chunks; ++c) {
-            const double w = mass[2 * c + which];
-            if (w > 0) { last = c; last_before = cum; }
-            if (cum + w > r) { at = c; before = cum; break; }
-            cum += w;
+        for (int c0 = 0; c0 < p.chunks && at < 0; c0 += 64) {
+            const double w = c0 + lane < p.chunks ? mass[2 * (c0 + lane) + which] : 0.0;
+            for (int k = 0; k < min(64, p.chunks - c0); ++k) {
+                const double wk = __shfl(w, k, 64);
+                if (wk > 0) { last = c0 + k; last_before = cum; }
+                if (cum + wk > r) { at = c0 + k; before = cum; break; }
+                cum += wk;
+            }
         }
-        s_chunk = at < 0 ? last : at;
-        s_r = r - (at < 0 ? last_before : before);
-        s_next = 0x7fffffff;
+        if (lane == 0) {
+            s_chunk = at < 0 ? last : at;
+            s_r = r - (at < 0 ? last_before : before);
+            s_next = 0x7fffffff;
+        }
     }
     __syncthreads();
     const int j0 = s_chunk * CHUNK, V = p.V, b0 = j0 + tid * PER;
@@ -303,16 +310,29 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
     const T* qrow = (const T*)p.draft + (long)b * p.d_sB + (long)ch.acc * p.d_sN;
     const int mode = which ? 0 : ch.mode, point = mode == 2 ? p.drafted[(long)b * p.N + ch.acc] : -1;
     // a thread's 16 scores follow one another here, so that its weights can be added up in order
+    constexpr int VEC = Piece<T>::VEC;
+    auto run_of = [&](const T* from, float* x) {
+#pragma unroll
+        for (int k = 0; k < PER; k += VEC) {
+            if (b0 + k + VEC <= V) {
+                const typename Piece<T>::V v = *(const typename Piece<T>::V*)(from + b0 + k);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[k + e] = widen(v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[k + e] = b0 + k + e < V ? to_f32<T>(from[b0 + k + e]) : (p.probs ? 0.f : -INFINITY);
+            }
+        }
+    };
+    float x[PER], y[PER];
+    run_of(row, x);
+    if (mode == 1) run_of(qrow, y);
     double w[PER], sum = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-        const int j = b0 + k;
-        double v = 0;
-        if (j < V) {
-            v = p.probs ? (double)to_f32<T>(row[j]) : exp_neg(((double)to_f32<T>(row[j]) - (double)ch.mp) * p.inv_t) / ch.zp;
-            if (mode == 1) v = fmax(v - (p.probs ? (double)to_f32<T>(qrow[j]) : exp_neg(((double)to_f32<T>(qrow[j]) - (double)ch.mq) * p.inv_t) / ch.zq), 0.0);
-            if (j == point) v = 0;
-        }
+        double v = probability(p, x[k], ch.mp, ch.rp);
+        if (mode == 1) v = fmax(v - probability(p, y[k], ch.mq, ch.rq), 0.0);
+        if (b0 + k == point) v = 0;
         w[k] = v;
         sum += v;
     }
