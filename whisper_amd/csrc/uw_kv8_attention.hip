@@ -13,17 +13,19 @@ namespace {
 //   S^T = K Q^T    16x16x32 MFMA, A = K codes as bf16 (exact), B = Q; lane (row = lane & 15, g = lane >> 4) gets for tile t the keys
 //                  16 g + 4 t + 0..3, because row slot r of tile t holds key 16 (r >> 2) + 4 t + (r & 3)
 //   O^T = V^T P^T  A = V codes as they lie (16 consecutive keys 16 g .. of one channel), B = P straight from those lanes
-// so neither K nor V nor P passes through LDS.  Scales multiply the scores (K) and the probabilities (V) -- one per 16 keys at
-// least, so one per lane.  Running maximum, sum and output in f32.  f32 queries and probabilities enter as three bf16 planes (24
-// bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.  bf16 queries are exact; their probabilities are
-// rounded to bf16 (2^-9 of each, independently), which is what the output is rounded to anyway.
+// so neither K nor V nor P passes through LDS.  K scales multiply the scores, V scales ride in the exponent of the weights; one per 16
+// keys at least, so one per lane.  References, sums and outputs are f32.
+//
+// bf16 queries enter exactly.  Their weights are rounded once to f16 for P V -- 2^-12 of each, and 2^-25 of the largest where they run
+// out of exponent -- an eighth of what the bf16 result is rounded by; the codes are exact in f16 too.  f32 queries and weights enter as
+// three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.
 struct AttnArgs {
     Kv8View c;
     TokSpan ts;
     TokArg q, o;
     float* lse;
     const int32_t* kv_len;
-    float* part;         // [rows][H][n_split][D + 4] partial results (output, maximum, sum) when n_split > 1
+    float* part;         // [rows][H][n_split][D + 4] partial results (output, its reference, sum, its reference) when n_split > 1
     int H, G, causal;
     int n_split;         // 1: an item is a row tile of a sequence; else at most so many items share a tile, each with a part of the keys
     int target, min_chunk;   // n_split > 1: items a head should come to, and the fewest blocks of 64 keys of one
@@ -59,6 +61,33 @@ template <> __device__ __forceinline__ bf16x8 codes8<UW_KV8_INT8>(unsigned a, un
     return v;
 }
 
+// the same in f16.  int8: 1024 + (code + 128) is f16 0x6400 | byte, so two bytes become two values by one byte permute and one packed
+// subtraction
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+template <int F> __device__ __forceinline__ f16x8 codes8h(unsigned a, unsigned b);
+template <> __device__ __forceinline__ f16x8 codes8h<UW_KV8_E4M3>(unsigned a, unsigned b)
+{
+    union { f16x2 p[4]; f16x8 v; } u;
+    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
+    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+    return u.v;
+}
+template <> __device__ __forceinline__ f16x8 codes8h<UW_KV8_INT8>(unsigned a, unsigned b)
+{
+    union { f16x2 p[4]; f16x8 v; } u;
+    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    u.p[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400)) - off;
+    u.p[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402)) - off;
+    u.p[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400)) - off;
+    u.p[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402)) - off;
+    return u.v;
+}
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // the planes of 8 f32 values
@@ -127,23 +156,34 @@ __device__ __forceinline__ float across_groups_max(float x)
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
+// what a wave, a workgroup or an item knows of a row beside its output
+struct RowState { float m, l, ms; };
+
+__device__ __forceinline__ void result_of(const RowState& a, float& factor, float& lse)
+{
+    // out = o 2^(m - ms) / l; a row that saw no key has l = 0
+    factor = a.l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a.m - a.ms) / a.l;
+    lse = a.l == 0.f ? -INFINITY : a.ms * LN2 + logf(a.l);
+}
+
 // four channels of a finished row (or of a split's part of it)
 template <typename T, int D>
-__device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first, int kvh, int row, int d, int split, int splits, float M, float L, f32x4 acc)
+__device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first, int kvh, int row, int d, int split, int splits, RowState a, f32x4 acc)
 {
     const int t = row / p.G, h = kvh * p.G + row % p.G;
     const long rg = t_first + t;                        // row of the call
     if (splits > 1) {
         float* at = p.part + ((rg * p.H + h) * p.n_split + split) * (D + 4);
         *(f32x4*)(at + d) = acc;
-        if (d == 0) { at[D] = M; at[D + 1] = L; }
+        if (d == 0) { at[D] = a.m; at[D + 1] = a.l; at[D + 2] = a.ms; }
         return;
     }
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    float factor, lse;
+    result_of(a, factor, lse);
     T* out = (T*)p.o.data + (p.ts.tok_start ? rg * p.o.sT : (long)b * p.o.sB + (long)t * p.o.sT) + (long)h * p.o.sH + d;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(acc[k] * inv);
-    if (p.lse && d == 0) p.lse[rg * p.H + h] = L == 0.f ? -INFINITY : M * LN2 + logf(L);
+    for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(acc[k] * factor);
+    if (p.lse && d == 0) p.lse[rg * p.H + h] = lse;
 }
 
 // WK waves share the keys of a row tile (their results are joined in LDS), WR row tiles per workgroup
@@ -157,7 +197,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
     constexpr unsigned STAGE_BYTES = 64 * D * 2;
-    static_assert(!RING || (WR == 4 && WK == 1), "a ring is filled and read by four waves of rows");
+    static_assert(WR == 1 || WK == 1, "waves share keys or stand side by side on rows");
+    static_assert(!RING || WR == 4, "a ring is filled and read by four waves of rows");
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % WK, wr = wave / WK;
     const int rr = lane & 15, g4 = lane >> 4;
@@ -224,10 +265,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     }
 
     f32x4 o[RT][D / 16];
-    float m[RT], l[RT];
+    float m[RT], l[RT], ms[RT];        // o holds weights * 2^-m, l weights * 2^-ms without the V scales (all in powers of two)
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        m[i] = -INFINITY;
+        m[i] = ms[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) o[i][d] = f32x4{0, 0, 0, 0};
@@ -332,10 +373,9 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        // a block of zeros (scale 0) has codes of zero: any scale does.  The V scale rides in the exponent: p' = p * vs costs nothing per
-        // element, the sum is divided by it once per block (the rounding of log2(vs) adds |log2 vs| 2^-24 to an element)
-        const float vsc = vs == 0.f ? 1.f : vs, lv = __builtin_amdgcn_logf(vsc), iv = __builtin_amdgcn_rcpf(vsc);
-        bf16x8 pf[RT][2][NP];
+        // a block of zeros (scale 0) has codes of zero: any scale does.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
+        const float lv = __builtin_amdgcn_logf(vs == 0.f ? 1.f : vs);
+        typename std::conditional<NP == 1, f16x8, bf16x8>::type pf[RT][2][NP];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int left = lim[i] - jv;          // keys of this lane's 16 that the row sees
@@ -346,9 +386,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                     for (int e = 0; e < 4; ++e)
                         if (4 * t + e >= left) st[i][t][e] = -INFINITY;
             }
-            float x[16], sum;
-            auto weigh = [&](float base) {
+            float x[16], sum, unit;
+            auto weigh = [&](float base, float base_s) {
                 const float nb = lv - base;
+                unit = __builtin_amdgcn_exp2f((base - base_s) - lv);      // what the sum of x counts in l
 #pragma unroll
                 for (int k = 0; k < 16; ++k) x[k] = __builtin_amdgcn_exp2f(fmaf(st[i][k >> 2][k & 3], kscale, nb));
                 if constexpr (mask) {                            // a scale behind the end may be NaN
@@ -360,33 +401,39 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
                 for (int k = 1; k < 16; ++k) sum += x[k];
             };
-            // The reference that scores are taken against need not be the largest so far, only near it: it moves when a lane's 16
-            // weights add up to more than 2^10 (at the first block it is -inf, the sum +inf), so that most blocks look for no maximum
-            // and rescale nothing.  Weights stay below 2^10, sums and outputs in f32; bf16 keeps its 8 bits at any size.
+            // The references need not be the largest so far, only near it: they move when a lane's 16 weights add up to more than 2^10 (at
+            // the first block they are -inf, the sum +inf), so that most blocks look for no maximum and rescale nothing.
             bool follow = true;
             if constexpr (!mask) {
-                weigh(m[i]);
-                follow = __any(sum * iv > 1024.f);
+                weigh(m[i], ms[i]);
+                follow = __any(sum > 0x1p10f || sum * unit > 0x1p60f);
             }
             if (follow) {
+                if constexpr (!mask) asm volatile("");           // rare: nothing of it belongs in front of the branch
                 float mx = fmaxf(st[i][0][0], st[i][0][1]);
 #pragma unroll
                 for (int k = 2; k < 16; k += 2) mx = fmaxf(fmaxf(mx, st[i][k >> 2][k & 3]), st[i][k >> 2][(k & 3) + 1]);
                 mx *= kscale;
                 if (mask && left <= 0) mx = -INFINITY;      // nothing of these 16 keys is seen, and the scale may be any leftover
-                mx = across_groups_max(mx);
-                const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;
+                const float mn = fmaxf(m[i], across_groups_max(mx + lv)), msn = fmaxf(ms[i], across_groups_max(mx));
+                const float base = mn == -INFINITY ? 0.f : mn, base_s = msn == -INFINITY ? 0.f : msn;
                 const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
-                l[i] *= alpha;
+                l[i] *= __builtin_amdgcn_exp2f(ms[i] - base_s);
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) o[i][d] *= alpha;
                 m[i] = mn;
-                weigh(base);
+                ms[i] = msn;
+                weigh(base, base_s);
             }
             // (a poisoned scale of a block that is seen shows in the sum)
-            if (!mask || left > 0) l[i] = fmaf(sum, iv, l[i]);
-            planes<NP>(x, pf[i][0]);
-            planes<NP>(x + 8, pf[i][1]);
+            if (!mask || left > 0) l[i] = fmaf(sum, unit, l[i]);
+            if constexpr (NP == 1) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) pf[i][k >> 3][0][k & 7] = (_Float16)x[k];
+            } else {
+                planes<NP>(x, pf[i][0]);
+                planes<NP>(x + 8, pf[i][1]);
+            }
         }
         if constexpr (RING) {
             const uint4* from = ring + (blk % STAGES) * (STAGE_BYTES / 16) + 4 * HALF * 64 + lane;
@@ -400,7 +447,14 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         }
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            const bf16x8 a0 = codes8<F>(vf[d].x, vf[d].y), a1 = codes8<F>(vf[d].z, vf[d].w);
+            typename std::conditional<NP == 1, f16x8, bf16x8>::type a0, a1;
+            if constexpr (NP == 1) {
+                a0 = codes8h<F>(vf[d].x, vf[d].y);
+                a1 = codes8h<F>(vf[d].z, vf[d].w);
+            } else {
+                a0 = codes8<F>(vf[d].x, vf[d].y);
+                a1 = codes8<F>(vf[d].z, vf[d].w);
+            }
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -452,14 +506,13 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     // join the waves that shared the keys
     if constexpr (WK > 1) {
         const int R = p.lds_rows;
-        float* sm = lds + (long)wr * WK * R * (D + 2);                    // [WK][R] m, [WK][R] l, [WK][R][D]
-        float* sl = sm + WK * R;
-        float* so = sl + WK * R;
+        RowState* sr = (RowState*)lds;                                    // [WK][R]
+        float* so = lds + WK * R * 3;                                     // [WK][R][D]
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int r = 16 * i + rr;
             if (r >= R) continue;
-            if (g4 == 0) { sm[wk * R + r] = m[i]; sl[wk * R + r] = l[i]; }
+            if (g4 == 0) sr[wk * R + r] = RowState{m[i], l[i], ms[i]};
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
                 float* at = so + ((long)wk * R + r) * D + d * 16 + g4 * 4;
@@ -469,18 +522,22 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         __syncthreads();
         for (int e = (wk * 64 + lane) * 4; e < (row_end - row0) * D; e += 64 * WK * 4) {
             const int r = e / D, d = e % D;
-            float M = -INFINITY, L = 0.f;
+            RowState a = {-INFINITY, 0.f, -INFINITY};
             f32x4 acc = {0, 0, 0, 0};
-            for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[w * R + r]);
+            for (int w = 0; w < WK; ++w) {
+                a.m = fmaxf(a.m, sr[w * R + r].m);
+                a.ms = fmaxf(a.ms, sr[w * R + r].ms);
+            }
             for (int w = 0; w < WK; ++w) {
                 // a wave without a finite score has a sum of 0, or NaN where it met a NaN
-                const float mw = sm[w * R + r], f = mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - M);
-                L += sl[w * R + r] * f;
-                const float* x = so + ((long)w * R + r) * D + d;
+                const RowState x = sr[w * R + r];
+                a.l += x.l * (x.ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.ms - a.ms));
+                const float f = x.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.m - a.m);
+                const float* y = so + ((long)w * R + r) * D + d;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] += x[k] * f;
+                for (int k = 0; k < 4; ++k) acc[k] += y[k] * f;
             }
-            store_row<T, D>(p, b, t_first, kvh, row0 + r, d, split, splits, M, L, acc);
+            store_row<T, D>(p, b, t_first, kvh, row0 + r, d, split, splits, a, acc);
         }
     } else {
 #pragma unroll
@@ -488,7 +545,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             const int row = row0 + 16 * i + rr;
             if (row < n_rows)
 #pragma unroll
-                for (int d = 0; d < D / 16; ++d) store_row<T, D>(p, b, t_first, kvh, row, d * 16 + g4 * 4, split, splits, m[i], l[i], o[i][d]);
+                for (int d = 0; d < D / 16; ++d) store_row<T, D>(p, b, t_first, kvh, row, d * 16 + g4 * 4, split, splits, RowState{m[i], l[i], ms[i]}, o[i][d]);
         }
     }
 }
@@ -518,22 +575,28 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p, int tile_rows
     const int splits = splits_of(p, b, chunk_of(p, tile_rows));
     if (splits == 1) return;                         // its workgroup wrote the result
     const float* part = p.part + w * p.n_split * (D + 4);
-    float M = -INFINITY, L = 0.f, acc[D / 64] = {};
-    for (int s = lane; s < splits; s += 64) M = fmaxf(M, part[s * (D + 4) + D]);
-    M = wave_max(M);
+    RowState a = {-INFINITY, 0.f, -INFINITY};
+    float acc[D / 64] = {};
+    for (int s = lane; s < splits; s += 64) {
+        a.m = fmaxf(a.m, part[s * (D + 4) + D]);
+        a.ms = fmaxf(a.ms, part[s * (D + 4) + D + 2]);
+    }
+    a.m = wave_max(a.m);
+    a.ms = wave_max(a.ms);
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         const float* x = part + s * (D + 4);
-        const float ms = x[D], ls = x[D + 1];
-        const float f = ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms - M);
-        L += ls * f;
+        const RowState o = {x[D], x[D + 1], x[D + 2]};
+        a.l += o.l * (o.ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(o.ms - a.ms));
+        const float f = o.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(o.m - a.m);
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) acc[k] += x[k * 64 + lane] * f;
     }
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    float factor, lse;
+    result_of(a, factor, lse);
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k) ((T*)p.o.data)[oat + (long)h * p.o.sH + k * 64 + lane] = from_f32<T>(acc[k] * inv);
-    if (p.lse && lane == 0) p.lse[row * p.H + h] = L == 0.f ? -INFINITY : M * LN2 + logf(L);
+    for (int k = 0; k < D / 64; ++k) ((T*)p.o.data)[oat + (long)h * p.o.sH + k * 64 + lane] = from_f32<T>(acc[k] * factor);
+    if (p.lse && lane == 0) p.lse[row * p.H + h] = lse;
 }
 
 // ---- host side --------------------------------------------------------------------------------------
@@ -601,7 +664,7 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
 
 template <int F, typename T, int D, int RT, int WK, int WR, bool RING> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
 {
-    const size_t lds = RING ? (size_t)STAGES * 64 * D * 2 : WK > 1 ? (size_t)WR * WK * p.lds_rows * (D + 2) * 4 : 0;
+    const size_t lds = RING ? (size_t)STAGES * 64 * D * 2 : WK > 1 ? (size_t)WK * p.lds_rows * (D + 3) * 4 : 0;
     if (lds > 64 * 1024) {
         static PerDeviceFlag flag;
         if (flag.pending()) {
