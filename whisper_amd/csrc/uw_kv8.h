@@ -164,6 +164,48 @@ template <typename CNT> __device__ __forceinline__ bool locate(int idx, int B, C
     return false;
 }
 
+// The idx-th (sequence, part) pair when parts are dealt round by round from the sequences' ends: every sequence's last part, then every
+// second to last one, ...  (of causal queries the last parts are the longest).  Up to 256 sequences; j_out counts from the end.
+template <typename CNT> __device__ __forceinline__ bool locate_from_end(int idx, int B, CNT cnt, int& b_out, int& j_out)
+{
+    const int lane = threadIdx.x & 63;
+    int n[4] = {0, 0, 0, 0}, most = 0;
+    if (lane * 4 < B) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = cnt(min(lane * 4 + i, B - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (lane * 4 + i >= B) n[i] = 0;
+            most = max(most, n[i]);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    // parts of the first r rounds
+    auto dealt = [&](int r) { return __builtin_amdgcn_readlane(wave_scan((min(n[0], r) + min(n[1], r)) + (min(n[2], r) + min(n[3], r))), 63); };
+    if (dealt(most) <= idx) return false;
+    int lo = 0, hi = most;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (dealt(mid) <= idx) lo = mid;
+        else hi = mid;
+    }
+    int k = idx - dealt(lo);
+    const int own = (n[0] > lo) + (n[1] > lo) + (n[2] > lo) + (n[3] > lo), incl = wave_scan(own);
+    const int w = __ffsll((long long)__ballot(incl > k)) - 1;
+    k -= __builtin_amdgcn_readlane(incl - own, w);
+    int b = w * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int has = __builtin_amdgcn_readlane(n[i], w) > lo ? 1 : 0;
+        if (has && k == 0) b_out = b + i;
+        k -= has;
+    }
+    b_out = __builtin_amdgcn_readfirstlane(b_out);
+    j_out = lo;
+    return true;
+}
+
 // ---- host side: what every entry checks -----------------------------------------------------------------
 #define RUN(x)                   \
     do {                         \
