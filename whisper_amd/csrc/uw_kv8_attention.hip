@@ -140,13 +140,6 @@ template <bool ONCE> __device__ __forceinline__ uint4 ld_codes(const void* p)
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-// a wave-uniform address, in scalar registers
-__device__ __forceinline__ const uint8_t* in_scalars(const uint8_t* p)
-{
-    const uint64_t u = (uint64_t)p;
-    return (const uint8_t*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)u) | (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32);
-}
-
 // largest of the four lanes that hold a row (lane & 15 alike), without a trip through LDS; a NaN loses
 __device__ __forceinline__ float across_groups_max(float x)
 {
@@ -188,17 +181,19 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
 
 // WK waves share the keys of a row tile (their results are joined in LDS), WR row tiles per workgroup
 //
-// RING (WR = 4, pages of 64 tokens or more): the waves work on the same block at the same time, and its codes are brought into LDS once
-// for all of them, STAGES - 1 blocks ahead, by the LDS DMA -- a quarter by each wave, no registers held while they are under way.
-constexpr int STAGES = 4;
-
-template <int F, typename T, int D, int RT, int WK, int WR, bool RING>
+// WR = 4: the four waves go through the same blocks together.  Each brings a quarter of a block's codes, turns them into operands and
+// lays them in LDS in the order the lanes hold them, so that a code is converted once for 64 * RT rows; operands are read back as
+// whole 1 KiB pieces, without bank conflicts.  Two buffers and one barrier a block: while block x is worked on, x + 1 is converted
+// and the codes of x + 2 are under way in eight registers.
+template <int F, typename T, int D, int RT, int WK, int WR>
 __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
-    constexpr unsigned STAGE_BYTES = 64 * D * 2;
+    constexpr bool SHARE = WR == 4;
+    constexpr int BUFFER = 64 * D * 4 / 16;            // SHARE: 16-byte pieces of a block's operands
+    typedef typename std::conditional<NP == 1, f16x8, bf16x8>::type vtype;
     static_assert(WR == 1 || WK == 1, "waves share keys or stand side by side on rows");
-    static_assert(!RING || WR == 4, "a ring is filled and read by four waves of rows");
+    static_assert(WR == 1 || WR == 4, "");
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % WK, wr = wave / WK;
     const int rr = lane & 15, g4 = lane >> 4;
@@ -319,23 +314,41 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(RT == 1)>(vp + d * 16 * c.P);
     };
-    // RING: a wave asks for its share of a block, straight into LDS in the order the lanes hold it; `stage` of block x is x mod STAGES
-    uint4* const ring = (uint4*)lds;
-    const unsigned ring_at = RING ? lds_addr_of(lds) : 0;
-    auto request = [&](int x) {
-        const int id = max(0, __builtin_amdgcn_readlane(w_id, at_key(x << 6)));
-        const int in_page = (x << 6) & (c.P - 1);
-        const long at = ((long)id * c.Hkv + kvh) * page_bytes;
-        const uint8_t* kp = in_scalars(c.k + at + in_page * D);
-        const uint8_t* vp = in_scalars(c.v + at + in_page);
-        const unsigned to = ring_at + (unsigned)(x % STAGES) * STAGE_BYTES;
+    auto v_operand = [&](unsigned x, unsigned y) {
+        if constexpr (NP == 1) return codes8h<F>(x, y);
+        else return codes8<F>(x, y);
+    };
+    // SHARE: this wave's quarter of a block -- K tile wr, every fourth V tile from wr on
+    bf16x8* const k_ops = (bf16x8*)lds;                // [2 buffers][BUFFER / 2 of K, then as many of V]
+    vtype* const v_ops = (vtype*)lds;
+    uint4 raw[2 * HALF];
+    auto bring = [&](int x) {
+        const int jk = (x << 6) + k_group, jv = (x << 6) + 16 * g4;
+        const int ik = max(0, __shfl(w_id, at_key(jk), 64)), iv = max(0, __shfl(w_id, at_key(jv), 64));
+        const uint8_t* kp = c.k + ((long)ik * c.Hkv + kvh) * page_bytes + ((jk & (c.P - 1)) + k_in + 4 * wr) * D + g4 * 16;
+        const uint8_t* vp = c.v + ((long)iv * c.Hkv + kvh) * page_bytes + (wr * 16 + rr) * c.P + (jv & (c.P - 1));
 #pragma unroll
         for (int hf = 0; hf < HALF; ++hf) {
-            glds16_sv(kp, (unsigned)((k_group + k_in + 4 * wr) * D + hf * 64 + g4 * 16), to + (wr * HALF + hf) * 1024);
-            glds16_sv(vp, (unsigned)(((hf * 4 + wr) * 16 + rr) * c.P + g4 * 16), to + (4 * HALF + hf * 4 + wr) * 1024);
+            raw[hf] = ld_codes<false>(kp + hf * 64);
+            raw[HALF + hf] = ld_codes<false>(vp + hf * 64 * c.P);
         }
     };
-    if (!RING && blk < blk1) {
+    auto convert = [&](int x) {
+        const int to = (x & 1) * BUFFER + lane;
+        if (len - (x << 6) < 64) {      // leftovers behind the sequence's end may hold NaN, which a weight of 0 does not silence
+            const int keep = max(0, min(16, len - ((x << 6) + 16 * g4)));
+#pragma unroll
+            for (int hf = 0; hf < HALF; ++hf) raw[HALF + hf] = first_bytes(raw[HALF + hf], keep);
+        }
+#pragma unroll
+        for (int hf = 0; hf < HALF; ++hf) {
+            k_ops[to + ((wr * HALF + hf) * 2) * 64] = codes8<F>(raw[hf].x, raw[hf].y);
+            k_ops[to + ((wr * HALF + hf) * 2 + 1) * 64] = codes8<F>(raw[hf].z, raw[hf].w);
+            v_ops[to + BUFFER / 2 + ((hf * 4 + wr) * 2) * 64] = v_operand(raw[HALF + hf].x, raw[HALF + hf].y);
+            v_ops[to + BUFFER / 2 + ((hf * 4 + wr) * 2 + 1) * 64] = v_operand(raw[HALF + hf].z, raw[HALF + hf].w);
+        }
+    };
+    if (!SHARE && blk < blk1) {
         window(blk);
         load_k(blk);
         load_v(blk);
@@ -344,16 +357,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool mask = decltype(masked)::value;
         const int j0 = blk << 6, jv = j0 + 16 * g4;
-        const bool more = !RING && blk + WK < blk1;
+        const bool more = !SHARE && blk + WK < blk1;
         const float kscale = __shfl(w_ks, at_key(jv), 64), vs = __shfl(w_vs, at_key(jv), 64);
         if (more && !in_window(blk + WK)) window(blk + WK);
-        if constexpr (RING) {
-            const uint4* from = ring + (blk % STAGES) * (STAGE_BYTES / 16) + lane;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = from[(t * HALF + hf) * 64];
-        }
+        const int from = (blk & 1) * BUFFER + lane;      // SHARE
 
         f32x4 st[RT][4];
 #pragma unroll
@@ -364,7 +371,14 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int hf = 0; hf < HALF; ++hf) {
-                const bf16x8 a0 = codes8<F>(kf[t][hf].x, kf[t][hf].y), a1 = codes8<F>(kf[t][hf].z, kf[t][hf].w);
+                bf16x8 a0, a1;
+                if constexpr (SHARE) {
+                    a0 = k_ops[from + ((t * HALF + hf) * 2) * 64];
+                    a1 = k_ops[from + ((t * HALF + hf) * 2 + 1) * 64];
+                } else {
+                    a0 = codes8<F>(kf[t][hf].x, kf[t][hf].y);
+                    a1 = codes8<F>(kf[t][hf].z, kf[t][hf].w);
+                }
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -373,7 +387,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                         st[i][t] = mfma(a1, qf[i][hf][1][pl], st[i][t]);
                     }
             }
-        if constexpr (!RING) {
+        if constexpr (!SHARE) {
             __builtin_amdgcn_sched_barrier(0);
             if (more) load_k(blk + WK);          // in flight under the softmax and P.V
             __builtin_amdgcn_sched_barrier(0);
@@ -381,7 +395,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 
         // a block of zeros (scale 0) has codes of zero: any scale does.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
         const float lv = __builtin_amdgcn_logf(vs == 0.f ? 1.f : vs);
-        typename std::conditional<NP == 1, f16x8, bf16x8>::type pf[RT][2][NP];
+        vtype pf[RT][2][NP];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int left = lim[i] - jv;          // keys of this lane's 16 that the row sees
@@ -441,25 +455,20 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                 planes<NP>(x + 8, pf[i][1]);
             }
         }
-        if constexpr (RING) {
-            const uint4* from = ring + (blk % STAGES) * (STAGE_BYTES / 16) + 4 * HALF * 64 + lane;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) vf[d] = from[d * 64];
-        }
-        if constexpr (mask) {      // leftovers behind the sequence's end may hold NaN, which a probability of 0 does not silence
+        if constexpr (mask && !SHARE) {      // leftovers behind the sequence's end may hold NaN, which a weight of 0 does not silence
             const int keep = max(0, min(16, len - jv));
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) vf[d] = first_bytes(vf[d], keep);
         }
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            typename std::conditional<NP == 1, f16x8, bf16x8>::type a0, a1;
-            if constexpr (NP == 1) {
-                a0 = codes8h<F>(vf[d].x, vf[d].y);
-                a1 = codes8h<F>(vf[d].z, vf[d].w);
+            vtype a0, a1;
+            if constexpr (SHARE) {
+                a0 = v_ops[from + BUFFER / 2 + (d * 2) * 64];
+                a1 = v_ops[from + BUFFER / 2 + (d * 2 + 1) * 64];
             } else {
-                a0 = codes8<F>(vf[d].x, vf[d].y);
-                a1 = codes8<F>(vf[d].z, vf[d].w);
+                a0 = v_operand(vf[d].x, vf[d].y);
+                a1 = v_operand(vf[d].z, vf[d].w);
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i)
@@ -469,7 +478,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                     o[i][d] = mfma(a1, pf[i][1][pl], o[i][d]);
                 }
         }
-        if constexpr (!RING) {
+        if constexpr (!SHARE) {
             __builtin_amdgcn_sched_barrier(0);
             if (more) load_v(blk + WK);
             __builtin_amdgcn_sched_barrier(0);
@@ -481,23 +490,28 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             else step(std::false_type{});
         }
     };
-    if constexpr (!RING) {
+    if constexpr (!SHARE) {
         steps(blk1);
     } else {
-        // the waves go through the blocks together, as far as the one that sees most; requests run STAGES - 1 blocks ahead
-        const int all_end = min((tile * WR + WR) * ROWS, n_rows);
+        // as far as the wave that sees most
+        const int all_end = min((tile + 1) * WR * ROWS, n_rows);
         const int most = all_end > 0 ? seen(all_end - 1) : 0, end = min((most >> 6) + ((most & 63) ? 1 : 0), p.max_blocks);
-        if (end > 0) window(0);
-        for (int x = 0; x < min(STAGES - 1, end); ++x) request(x);
+        if (end > 0) {
+            window(0);
+            bring(0);
+            convert(0);
+            if (end > 1) bring(1);
+        }
         for (blk = 0; blk < end;) {
-            // this block's pieces of this wave have landed when at most the later blocks' are under way; then everybody's have.  Whoever
-            // passes the barrier is done with block blk - 1, whose stage the next request takes.
-            if (blk + STAGES - 1 < end) __builtin_amdgcn_s_waitcnt(0x0F70 | ((STAGES - 2) * 2 * HALF));
-            else __builtin_amdgcn_s_waitcnt(0x0F70);
+            // this wave's pieces of block blk are in LDS, then everybody's; whoever is here is done with block blk - 1, whose buffer is
+            // written next
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (blk + STAGES - 1 < end) {
-                if (!in_window(blk + STAGES - 1)) window(blk);
-                request(blk + STAGES - 1);
+            if (blk + 1 < end) {
+                convert(blk + 1);
+                if (blk + 2 < end) {
+                    if (!in_window(blk + 2)) window(blk);
+                    bring(blk + 2);
+                }
             }
             if (blk < blk1) steps(blk + 1);
             else ++blk;
@@ -622,7 +636,6 @@ constexpr int max_row_tiles(size_t elem, int D) { return elem == 4 && D == 128 ?
 
 struct AttnPlan {
     int rt, wk, wr;      // row tiles of 16 per wave, waves sharing keys, waves side by side on rows
-    bool ring;
     int n_split, target, min_chunk, tiles, max_blocks, lds_rows;
     long groups, ws_bytes;
 };
@@ -647,7 +660,6 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
         p.wk = 1;
         p.wr = 4;
     }
-    p.ring = p.wr == 4 && c->page >= 64;
     const int per = 16 * p.rt * p.wr;
     p.tiles = T > 0 ? ceil_div(rows, per) : 0;
     p.groups = T > 0 ? (long)B * p.tiles : n_tok * G / per + std::min((long)B, (long)n_tok);
@@ -668,17 +680,17 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     return p;
 }
 
-template <int F, typename T, int D, int RT, int WK, int WR, bool RING> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+template <int F, typename T, int D, int RT, int WK, int WR> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
 {
-    const size_t lds = RING ? (size_t)STAGES * 64 * D * 2 : WK > 1 ? (size_t)WK * p.lds_rows * (D + 3) * 4 : 0;
+    const size_t lds = WR == 4 ? (size_t)2 * 64 * D * 4 : WK > 1 ? (size_t)WK * p.lds_rows * (D + 3) * 4 : 0;
     if (lds > 64 * 1024) {
         static PerDeviceFlag flag;
         if (flag.pending()) {
-            UW_HIP_CHECK(hipFuncSetAttribute((const void*)kv8_attention_kernel<F, T, D, RT, WK, WR, RING>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            UW_HIP_CHECK(hipFuncSetAttribute((const void*)kv8_attention_kernel<F, T, D, RT, WK, WR>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
             flag.mark();
         }
     }
-    hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR, RING>), dim3((unsigned)(p.groups * a.c.Hkv)), dim3(64 * WK * WR), lds, s, a);
+    hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR>), dim3((unsigned)(p.groups * a.c.Hkv)), dim3(64 * WK * WR), lds, s, a);
     UW_LAUNCH_CHECK();
     return UW_OK;
 }
@@ -686,12 +698,11 @@ template <int F, typename T, int D, int RT, int WK, int WR, bool RING> int launc
 template <int F, typename T, int D> int launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
 {
     constexpr int RT = max_row_tiles(sizeof(T), D);
-    if (p.ring) return launch_attention_as<F, T, D, RT, 1, 4, true>(a, p, s);
-    if (p.wr == 4) return launch_attention_as<F, T, D, RT, 1, 4, false>(a, p, s);
-    if (p.wk == 8) return launch_attention_as<F, T, D, 1, 8, 1, false>(a, p, s);
-    if (p.rt == 1) RUN((launch_attention_as<F, T, D, 1, 4, 1, false>(a, p, s)));
+    if (p.wr == 4) return launch_attention_as<F, T, D, RT, 1, 4>(a, p, s);
+    if (p.wk == 8) return launch_attention_as<F, T, D, 1, 8, 1>(a, p, s);
+    if (p.rt == 1) RUN((launch_attention_as<F, T, D, 1, 4, 1>(a, p, s)));
     if constexpr (RT > 1) {
-        if (p.rt == RT) RUN((launch_attention_as<F, T, D, RT, 4, 1, false>(a, p, s)));
+        if (p.rt == RT) RUN((launch_attention_as<F, T, D, RT, 4, 1>(a, p, s)));
     }
     if (p.n_split == 1) return UW_OK;
     hipLaunchKernelGGL((kv8_join_kernel<T, D>), dim3(ceil_div(a.ts.N * a.H, 4)), dim3(256), 0, s, a, 16 * p.rt);
