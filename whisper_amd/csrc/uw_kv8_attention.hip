@@ -306,13 +306,13 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = ld_codes<(RT == 1)>(kp + t * 4 * D + hf * 64);
+            for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = ld_codes<(WR == 1)>(kp + t * 4 * D + hf * 64);
     };
     auto load_v = [&](int x) {
         const int j = (x << 6) + 16 * g4, id = max(0, __shfl(w_id, at_key(j), 64));
         const uint8_t* vp = c.v + ((long)id * c.Hkv + kvh) * page_bytes + rr * c.P + (j & (c.P - 1));
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(RT == 1)>(vp + d * 16 * c.P);
+        for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(WR == 1)>(vp + d * 16 * c.P);
     };
     auto v_operand = [&](unsigned x, unsigned y) {
         if constexpr (NP == 1) return codes8h<F>(x, y);
@@ -642,9 +642,13 @@ struct AttnPlan {
 
 // How a call is cut.
 //  - up to 16 rows of a kv head: one row tile, the waves share the keys
-//  - more: tiles of 128 rows, 32 to a wave, if there are enough of them to fill the chip; else tiles of 32 rows whose four waves share
-//    the keys -- four times the workgroups for the same rows
-//  - long sequences are cut further where the waves share the keys, into items of equal size (chunk_of), joined by a second launch
+//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), if that gives 384 workgroups; else tiles of 16 or 32
+//    rows whose four waves share the keys -- more workgroups for the same rows.  Measured (us, side by side / sharing keys): 170 rows x
+//    64 heads over 1500 keys 32 / 18, 2000 rows x 8 heads 38 / 17, 170 rows x 192 heads 45 / 46, the 33380 rows of 12 heads over
+//    5000 keys 168 / 240.  Of the latter, tiles of 16 rows where a row is short (64 channels: 16 against 18 us, 32 against 36), of 32
+//    where keys are many bytes (2048 rows over 8192 keys of 128 channels: 184 against 107 us)
+//  - long sequences are cut further where the waves share the keys, into items of equal size (chunk_of), joined by a second launch.
+//    Short ones are not: up to 32 blocks, eight or four waves are through sooner than a second launch is
 AttnPlan plan_attention(const uw_kv8_attention_args* a)
 {
     AttnPlan p;
@@ -656,9 +660,13 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     p.rt = rows <= 16 ? 1 : max_row_tiles(a->seqs.dtype == UW_DTYPE_F32 ? 4 : 2, c->head_dim);
     p.wk = 4;
     p.wr = 1;
-    if (rows > 32 && (long)ceil_div(rows, 64 * p.rt) * B * c->n_kv_heads >= 384) {
-        p.wk = 1;
-        p.wr = 4;
+    if (rows > 32) {
+        if ((long)ceil_div(rows, 64 * p.rt) * B * c->n_kv_heads >= 384) {
+            p.wk = 1;
+            p.wr = 4;
+        } else if (c->head_dim == 64) {
+            p.rt = 1;
+        }
     }
     const int per = 16 * p.rt * p.wr;
     p.tiles = T > 0 ? ceil_div(rows, per) : 0;
