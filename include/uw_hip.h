@@ -47,6 +47,12 @@ int uw_ctx_destroy(uw_ctx* ctx);
 /* bytes of device memory the context holds */
 int64_t uw_ctx_bytes(const uw_ctx* ctx);
 
+/* Decode steps (uw_decode_step, uw_decode_greedy, uw_transcribe_windows) read the cross-attention K/V from an 8-bit copy that
+ * uw_cross_kv fills: format UW_KV8_INT8 or UW_KV8_E4M3, a scale per 64 frames and head (the paged cache below), or -1 for the compute
+ * dtype again.  It halves the stream that bounds a step; multi-token passes keep reading the compute dtype.  Allocates on its
+ * first use, synchronises, and asks for a new uw_cross_kv.  No counterpart in the reference. */
+int uw_ctx_cross_cache(uw_ctx* ctx, int format);
+
 /* Mel seam: calculate_mel_for_segment (urro_whisper/audio/load.py:67-121), i.e.
  * whisper.log_mel_spectrogram(audio, n_mels, padding=480000)[:, :3000].
  * audio: f32 [B][stride] 16 kHz PCM, n_samples: i32 [B] valid samples per window (<= stride),

@@ -107,6 +107,15 @@ def test_library_refuses_before_any_gpu_call():
         assert fn(None, None) > 0 and b"null arguments" in lib.uw_last_error()
 
 
+def test_cross_cache_refuses():
+    from whisper_amd.config import dims_for
+    from whisper_amd.engine import Engine
+    with pytest.raises(ValueError, match="cross_cache"):
+        Engine(dims_for("micro"), {}, cross_cache="int4")
+    lib = L.load()
+    assert lib.uw_ctx_cross_cache(None, L.UW_KV8_INT8) > 0 and b"null context" in lib.uw_last_error()
+
+
 def test_verify_draft_refuses():
     t, d, u = torch.zeros(2, 4, 10), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, 4)
     for kw, word in ((dict(target=t[0]), "target"), (dict(target=t.half()), "target"), (dict(target=t[:, :0]), "empty"),

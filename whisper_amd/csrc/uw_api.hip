@@ -108,6 +108,12 @@ struct uw_ctx {
     int32_t* split_ticket = nullptr;   // [Bm][H] arrival counters of the row-split cross-attention (zero between launches)
     int step_prefetch = -1;        // decode-step products request the following product's weights: -1 by row count, 0 never, 1 always
     int fused_logits = 1;          // up to 16 windows (bf16): LayerNorm + tied projection + arg-max candidates in one launch
+    // 8-bit copy of the cross K/V that decode steps read (uw_ctx_cross_cache); pages of 64 frames, window b's at b * cross8_width ...
+    int cross8_format = -1;        // -1: none, steps read cross_kv
+    uint8_t* cross8_codes = nullptr;   // [Ld][K | V][Bm * cross8_width][H][64 * 64]
+    float* cross8_scales = nullptr;    // [Ld][K | V][Bm * cross8_width][H]
+    int32_t *cross8_table = nullptr, *cross8_len = nullptr, *cross8_pos = nullptr;   // [Bm][cross8_width]; [Bm] frames; [Bm] zeros
+    int cross8_width = 0;
     float* cand_val = nullptr;     // [Bm rounded up to 16][uw_logits_rows16_blocks(V)] arg-max candidates of the step's logits
     int32_t* cand_idx = nullptr;
 };
@@ -576,6 +582,22 @@ size_t cross_kv_layer_bytes(const uw_ctx* c) { return (size_t)c->Bm * c->S * 2 *
 size_t cross_vt_layer_bytes(const uw_ctx* c) { return (size_t)c->Bm * c->d * c->Spad * c->es; }
 size_t self_kv_layer_bytes(const uw_ctx* c) { return (size_t)c->Bm * c->Tm * 2 * c->d * c->es; }
 
+uw_kv8_cache cross8_cache(const uw_ctx* c, size_t layer)
+{
+    const size_t pages = (size_t)c->Bm * c->cross8_width, codes = pages * c->H * 64 * 64, scales = pages * c->H;
+    uw_kv8_cache k = {};
+    k.k = c->cross8_codes + layer * 2 * codes;
+    k.v = c->cross8_codes + (layer * 2 + 1) * codes;
+    k.k_scale = c->cross8_scales + layer * 2 * scales;
+    k.v_scale = c->cross8_scales + (layer * 2 + 1) * scales;
+    k.n_pages = (int32_t)pages;
+    k.n_kv_heads = c->H;
+    k.page = 64;
+    k.head_dim = 64;
+    k.format = c->cross8_format;
+    return k;
+}
+
 int cross_kv_project(uw_ctx* c, int B, hipStream_t s)
 {
     const int d = c->d, S = c->S;
@@ -596,6 +618,15 @@ int cross_kv_project(uw_ctx* c, int B, hipStream_t s)
         // the V half also leaves transposed ([d][Spad] per window), the form the multi-token passes' attention reads
         p.C2 = vt; p.ldc2 = c->Spad; p.sC2 = (long)d * c->Spad; p.c2_col0 = d;
         RUN(uw_gemm(c->dt, 0, p, s));
+        if (c->cross8_format >= 0) {
+            uw_kv8_store_args a = {};
+            a.cache = cross8_cache(c, li);
+            a.seqs.table = c->cross8_table; a.seqs.len = c->cross8_pos; a.seqs.n_tok = (int64_t)B * S;
+            a.seqs.table_width = c->cross8_width; a.seqs.B = B; a.seqs.T = S; a.seqs.dtype = c->dt == UW_F32 ? UW_DTYPE_F32 : UW_DTYPE_BF16;
+            a.k.data = kv; a.k.seq_stride = (int64_t)S * 2 * d; a.k.tok_stride = 64; a.k.head_stride = (int64_t)S * 64;
+            a.v = a.k; a.v.data = (char*)kv + (size_t)S * d * c->es;
+            RUN(uw_kv8_append(&a, s));
+        }
     }
     c->cross_batch = B;
     return UW_OK;
@@ -795,7 +826,18 @@ int decoder_step_chunk(uw_ctx* c, int b0, int B, bool embed, bool greedy, hipStr
         cp.split_ticket = c->split_ticket + (long)b0 * H;
         const bool timed = c->prof_on && c->prof_used + 2 <= c->prof_ev.size();
         if (timed) UW_HIP_CHECK(hipEventRecord(c->prof_ev[c->prof_used], s));
-        RUN(uw_cross_attn_decode(c->dt, cp, s));
+        if (c->cross8_format >= 0) {
+            const uw_kv8_cache c8 = cross8_cache(c, li);
+            Kv8StepParams kp;
+            kp.cache = &c8; kp.table = c->cross8_table + (long)b0 * c->cross8_width; kp.width = c->cross8_width; kp.len = c->cross8_len + b0;
+            kp.q = qkv; kp.out = att; kp.out_lo = att_lo;
+            kp.rows = cp.rows; kp.rows_sB = cp.rows_sB; kp.rows_sSel = cp.rows_sSel; kp.row_index = cp.row_index; kp.active = active;
+            for (int h = 0; h < 32; ++h) kp.sel_slot[h] = cp.sel_slot[h];
+            kp.B = B; kp.S = S; kp.n_rows = Tm;
+            RUN(uw_kv8_cross_decode(c->dt, kp, s));
+        } else {
+            RUN(uw_cross_attn_decode(c->dt, cp, s));
+        }
         if (timed) { UW_HIP_CHECK(hipEventRecord(c->prof_ev[c->prof_used + 1], s)); c->prof_used += 2; }
         if (c->prof_on) { ++c->prof_launches; c->prof_windows += B; }
         RUN(gemm_step(c, att, att_lo, l.cross.wo_p, x, d, true, B, d, d, l.cross.bo, 0, x, d, false, s, &n_fc1));
@@ -973,6 +1015,32 @@ int uw_ctx_destroy(uw_ctx* c)
 }
 
 int64_t uw_ctx_bytes(const uw_ctx* c) { return c ? c->bytes : 0; }
+
+int uw_ctx_cross_cache(uw_ctx* c, int format)
+{
+    UW_REQUIRE(c, "uw_ctx_cross_cache: null context");
+    UW_REQUIRE(format == -1 || format == UW_KV8_INT8 || format == UW_KV8_E4M3, "uw_ctx_cross_cache: unknown format %d", format);
+    RUN(check_batch(c, 1));
+    if (format >= 0 && !c->cross8_codes) {
+        const int W = (c->S + 63) / 64;
+        const size_t pages = (size_t)c->Bm * W, Ld = c->dec.size();
+        // the host's tables first: nothing of the context changes before all of it is there
+        std::vector<int32_t> table(pages), len(c->Bm, c->S);
+        for (size_t i = 0; i < pages; ++i) table[i] = (int32_t)i;
+        ALLOC(c->cross8_scales, Ld * 2 * pages * c->H * 4, true);
+        ALLOC(c->cross8_table, pages * 4, false);
+        ALLOC(c->cross8_len, (size_t)c->Bm * 4, false);
+        ALLOC(c->cross8_pos, (size_t)c->Bm * 4, true);
+        UW_HIP_CHECK(hipMemcpy(c->cross8_table, table.data(), pages * 4, hipMemcpyHostToDevice));
+        UW_HIP_CHECK(hipMemcpy(c->cross8_len, len.data(), (size_t)c->Bm * 4, hipMemcpyHostToDevice));
+        c->cross8_width = W;
+        ALLOC(c->cross8_codes, Ld * 2 * pages * c->H * 64 * 64, true);
+        UW_HIP_CHECK(hipDeviceSynchronize());
+    }
+    if (format != c->cross8_format) c->cross_batch = 0;      // the next uw_cross_kv fills it
+    c->cross8_format = format;
+    return UW_OK;
+}
 
 int uw_profile_begin(uw_ctx* c, int max_launches)
 {

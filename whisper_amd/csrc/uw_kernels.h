@@ -211,6 +211,26 @@ int uw_greedy_next(int dtype, const GreedyState& st, const float* logits, long l
                    int ts_end, float* x, const float* tok_emb, const float* pos_emb, int d, hipStream_t s,
                    const float* cand_val = nullptr, const int32_t* cand_idx = nullptr, int n_cand = 0);
 
+// ---- uw_kv8_attention.hip -----------------------------------------------------------------------
+struct uw_kv8_cache;
+// cross-attention of one decoder step over an 8-bit paged cache: CrossDecodeParams with the cache in the place of K and V
+struct Kv8StepParams {
+    const uw_kv8_cache* cache = nullptr;  // this layer's
+    const int32_t* table = nullptr;       // [B][width] pages of each window
+    int width = 0;
+    const int32_t* len = nullptr;         // [B] keys of each window (at most S)
+    const void* q = nullptr;              // [B][d] scaled
+    void* out = nullptr;                  // [B][d] fragment-major
+    void* out_lo = nullptr;               // bf16: lo plane of the split output (see GemmParams)
+    float* rows = nullptr;                // attention rows [B][n_sel][n_rows][S] or null
+    long rows_sB = 0, rows_sSel = 0;
+    const int32_t* row_index = nullptr;
+    const int32_t* active = nullptr;
+    int sel_slot[32];                     // per head: slot in [n_sel] or -1
+    int B = 0, S = 0, n_rows = 0;
+};
+int uw_kv8_cross_decode(int dtype, const Kv8StepParams& p, hipStream_t s);
+
 // ---- uw_mel.hip -------------------------------------------------------------------------------
 struct MelTables;  // device tables owned by the context
 int uw_mel_tables_create(int n_mels, const float* filters_host /*[n_mels][201]*/, MelTables** out);

@@ -19,6 +19,19 @@ namespace {
 // bf16 queries enter exactly.  Their weights are rounded once to f16 for P V -- 2^-12 of each, and 2^-25 of the largest where they run
 // out of exponent -- an eighth of what the bf16 result is rounded by; the codes are exact in f16 too.  f32 queries and weights enter as
 // three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.
+// What a decoder step adds: one query token per window, its output in the operand layout of the product that follows, and the
+// probabilities of the alignment heads.
+struct StepArgs {
+    const int32_t* active;       // [B]; 0: the window is finished, nothing is written (or null)
+    void* out_lo;                // bf16: the plane of what rounding the output dropped (or null)
+    int d;                       // heads * 64
+    float* rows;                 // probabilities [B][slots][n_rows][S] (or null)
+    long rows_sB, rows_sSel;
+    const int32_t* row_index;    // [B] row to write, outside 0 .. n_rows-1: none
+    int n_rows, S;
+    signed char slot[32];        // per head, -1: not an alignment head
+};
+
 struct AttnArgs {
     Kv8View c;
     TokSpan ts;
@@ -34,6 +47,7 @@ struct AttnArgs {
     int lds_rows;        // rows of a tile that can be in use
     float scale2;        // |scale| * log2(e)
     unsigned neg;        // sign bit of scale, moved to the queries
+    StepArgs step;
 };
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -185,7 +199,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
 // lays them in LDS in the order the lanes hold them, so that a code is converted once for 64 * RT rows; operands are read back as
 // whole 1 KiB pieces, without bank conflicts.  Two buffers and one barrier a block: while block x is worked on, x + 1 is converted
 // and the codes of x + 2 are under way in eight registers.
-template <int F, typename T, int D, int RT, int WK, int WR>
+template <int F, typename T, int D, int RT, int WK, int WR, bool STEP>
 __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
@@ -194,6 +208,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     typedef typename std::conditional<NP == 1, f16x8, bf16x8>::type vtype;
     static_assert(WR == 1 || WK == 1, "waves share keys or stand side by side on rows");
     static_assert(WR == 1 || WR == 4, "");
+    static_assert(!STEP || (D == 64 && RT == 1 && WK > 1), "a decoder step has one row of a head");
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % WK, wr = wave / WK;
     const int rr = lane & 15, g4 = lane >> 4;
@@ -222,6 +237,19 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     } else {
         b = item % p.ts.B;
         tile = p.tiles - 1 - item / p.ts.B;
+    }
+    if (STEP && p.step.active && !p.step.active[b]) return;
+    // STEP: an alignment head's scores are kept in LDS (behind what the waves join there) until their sum is known
+    float *scores = nullptr, *row_out = nullptr;
+    if constexpr (STEP) {
+        const int slot = p.step.slot[kvh];
+        if (p.step.rows && slot >= 0) {
+            const int ri = p.step.row_index[b];
+            if (ri >= 0 && ri < p.step.n_rows) {
+                row_out = p.step.rows + (long)b * p.step.rows_sB + (long)slot * p.step.rows_sSel + (long)ri * p.step.S;
+                scores = lds + WK * (D + 3);
+            }
+        }
     }
     const int n = p.ts.count(b), n_rows = n * p.G;
     const int row0 = (tile * WR + wr) * ROWS;
@@ -406,6 +434,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                     for (int e = 0; e < 4; ++e)
                         if (4 * t + e >= left) st[i][t][e] = -INFINITY;
             }
+            if (STEP && scores && rr == 0) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) *(f32x4*)(scores + jv + 4 * t) = st[i][t] * kscale;
+            }
             float x[16], sum, unit;
             auto weigh = [&](float base, float base_s) {
                 const float nb = lv - base;
@@ -557,7 +589,27 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
                 for (int k = 0; k < 4; ++k) acc[k] += y[k] * f;
             }
-            store_row<T, D>(p, b, t_first, kvh, row0 + r, d, split, splits, a, acc);
+            if constexpr (STEP) {
+                float factor, lse;
+                result_of(a, factor, lse);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float v = acc[k] * factor;
+                    const T hi = from_f32<T>(v);
+                    const long at = frag_elem_offset<T>(b, kvh * 64 + d + k, p.step.d);
+                    ((T*)p.o.data)[at] = hi;
+                    if (p.step.out_lo) ((T*)p.step.out_lo)[at] = from_f32<T>(v - to_f32<T>(hi));
+                }
+            } else {
+                store_row<T, D>(p, b, t_first, kvh, row0 + r, d, split, splits, a, acc);
+            }
+        }
+        if (STEP && row_out) {
+            float ms0 = -INFINITY, l0 = 0.f;
+            for (int w = 0; w < WK; ++w) ms0 = fmaxf(ms0, sr[w].ms);
+            for (int w = 0; w < WK; ++w) l0 += sr[w].l * (sr[w].ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sr[w].ms - ms0));
+            const float inv = 1.0f / l0;
+            for (int j = tid; j < p.step.S; j += 64 * WK) row_out[j] = j < len ? __builtin_amdgcn_exp2f(scores[j] - ms0) * inv : 0.f;
         }
     } else {
 #pragma unroll
@@ -688,17 +740,18 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     return p;
 }
 
-template <int F, typename T, int D, int RT, int WK, int WR> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+template <int F, typename T, int D, int RT, int WK, int WR, bool STEP = false> int launch_attention_as(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
 {
-    const size_t lds = WR == 4 ? (size_t)2 * 64 * D * 4 : WK > 1 ? (size_t)WK * p.lds_rows * (D + 3) * 4 : 0;
+    size_t lds = WR == 4 ? (size_t)2 * 64 * D * 4 : WK > 1 ? (size_t)WK * p.lds_rows * (D + 3) * 4 : 0;
+    if (STEP && a.step.rows) lds += (size_t)p.max_blocks * 64 * 4;
     if (lds > 64 * 1024) {
         static PerDeviceFlag flag;
         if (flag.pending()) {
-            UW_HIP_CHECK(hipFuncSetAttribute((const void*)kv8_attention_kernel<F, T, D, RT, WK, WR>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            UW_HIP_CHECK(hipFuncSetAttribute((const void*)kv8_attention_kernel<F, T, D, RT, WK, WR, STEP>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
             flag.mark();
         }
     }
-    hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR>), dim3((unsigned)(p.groups * a.c.Hkv)), dim3(64 * WK * WR), lds, s, a);
+    hipLaunchKernelGGL((kv8_attention_kernel<F, T, D, RT, WK, WR, STEP>), dim3((unsigned)(p.groups * a.c.Hkv)), dim3(64 * WK * WR), lds, s, a);
     UW_LAUNCH_CHECK();
     return UW_OK;
 }
@@ -718,7 +771,59 @@ template <int F, typename T, int D> int launch_attention(const AttnArgs& a, cons
     return UW_OK;
 }
 
+template <int F, typename T> int launch_step(const AttnArgs& a, const AttnPlan& p, hipStream_t s)
+{
+    // few (window, head) pairs: more waves in each workgroup, as plan_attention has it
+    return p.groups * a.c.Hkv <= 256 ? launch_attention_as<F, T, 64, 1, 8, 1, true>(a, p, s) : launch_attention_as<F, T, 64, 1, 4, 1, true>(a, p, s);
+}
+
 }  // namespace
+
+int uw_kv8_cross_decode(int dtype, const Kv8StepParams& p, hipStream_t s)
+{
+    RUN(check_cache("kv8_cross_decode", p.cache));
+    UW_REQUIRE(p.cache->head_dim == 64 && p.cache->n_kv_heads <= 32 && p.B > 0 && p.q && p.out && p.table && p.len && p.width > 0, "kv8_cross_decode: bad arguments");
+    UW_REQUIRE(p.S > 0 && p.S <= 8192 && (long)p.width * p.cache->page >= p.S, "kv8_cross_decode: %d keys in %d pages", p.S, p.width);
+    UW_REQUIRE(!p.rows || p.row_index, "kv8_cross_decode: rows without row_index");
+    const int H = p.cache->n_kv_heads, d = H * 64;
+    UW_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.out) & 15) == 0, "kv8_cross_decode: misaligned operands");
+    uw_kv8_seqs seqs = {};
+    seqs.table = p.table;
+    seqs.table_width = p.width;
+    AttnArgs a = {};
+    a.c = view_of(p.cache, &seqs);
+    a.ts = TokSpan{nullptr, p.B, 1, p.B};
+    a.q = TokArg{(void*)p.q, d, d, 64};
+    a.o = TokArg{p.out, d, d, 64};
+    a.kv_len = p.len;
+    a.H = H;
+    a.G = 1;
+    a.n_split = 1;
+    a.tiles = 1;
+    a.groups = p.B;
+    a.lds_rows = 1;
+    a.scale2 = LOG2E;                 // queries come scaled
+    a.step.active = p.active;
+    a.step.out_lo = p.out_lo;
+    a.step.d = d;
+    bool any = false;
+    for (int h = 0; h < 32; ++h) {
+        a.step.slot[h] = (signed char)(h < H ? p.sel_slot[h] : -1);
+        any = any || a.step.slot[h] >= 0;
+    }
+    a.step.rows = any ? p.rows : nullptr;
+    a.step.rows_sB = p.rows_sB;
+    a.step.rows_sSel = p.rows_sSel;
+    a.step.row_index = p.row_index;
+    a.step.n_rows = p.n_rows;
+    a.step.S = p.S;
+    AttnPlan pl = {};
+    pl.groups = p.B;
+    pl.lds_rows = 1;
+    pl.max_blocks = a.max_blocks = ceil_div(p.S, 64);
+    if (p.cache->format == UW_KV8_INT8) return dtype == UW_BF16 ? launch_step<UW_KV8_INT8, bf16_t>(a, pl, s) : launch_step<UW_KV8_INT8, float>(a, pl, s);
+    return dtype == UW_BF16 ? launch_step<UW_KV8_E4M3, bf16_t>(a, pl, s) : launch_step<UW_KV8_E4M3, float>(a, pl, s);
+}
 
 extern "C" {
 
@@ -737,7 +842,7 @@ int uw_kv8_attention(const uw_kv8_attention_args* a, void* stream)
     UW_REQUIRE(pl.ws_bytes == 0 || (a->ws && ((uintptr_t)a->ws & 15) == 0 && a->ws_bytes >= pl.ws_bytes),
                "uw_kv8_attention: workspace missing, misaligned or smaller than %lld bytes", (long long)pl.ws_bytes);
     UW_REQUIRE(pl.groups * a->cache.n_kv_heads < (1 << 22) && q.n_tok * a->n_heads <= 0x7fffffff, "uw_kv8_attention: too many rows");
-    AttnArgs x;
+    AttnArgs x = {};
     x.c = view_of(&a->cache, &q);
     x.ts = span_of(&q);
     x.q = arg_of(&a->q);

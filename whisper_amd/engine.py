@@ -22,7 +22,10 @@ def _i32(x, device) -> torch.Tensor:
 class Engine:
     def __init__(self, dims: WhisperDims, state_dict: Dict[str, torch.Tensor], dtype: str = "bf16", max_batch: int = 1,
                  align_heads: Optional[Sequence[Tuple[int, int]]] = None, device: str = "cuda:0",
-                 n_text_ctx: Optional[int] = None):
+                 n_text_ctx: Optional[int] = None, cross_cache: Optional[str] = None):
+        """cross_cache: None, or "int8" / "e4m3": decode steps read the cross-attention K/V in 8 bits (see kv8.py)."""
+        if cross_cache is not None and cross_cache not in L.KV8_FORMATS:
+            raise ValueError(f"cross_cache must be None or one of {sorted(L.KV8_FORMATS)}, got {cross_cache!r}")
         if not torch.cuda.is_available():
             raise L.UwError("no GPU visible: the transcription path runs on MI355X only (no CPU fallback)")
         self.lib = L.load()
@@ -57,6 +60,8 @@ class Engine:
         torch.cuda.synchronize()
         L.check(self.lib.uw_ctx_create(C.byref(cfg), arr, len(dev_w), filt.ctypes.data_as(C.c_void_p), C.byref(handle)))
         self.ctx = handle
+        if cross_cache is not None:
+            L.check(self.lib.uw_ctx_cross_cache(self.ctx, L.KV8_FORMATS[cross_cache]))
         del dev_w
         torch.cuda.empty_cache()
 

@@ -17,6 +17,7 @@ UW_DTYPE_BF16 = 1
 UW_MAX_ALIGN_HEADS = 32
 UW_KV8_INT8 = 0
 UW_KV8_E4M3 = 1
+KV8_FORMATS = {"int8": UW_KV8_INT8, "e4m3": UW_KV8_E4M3}
 
 
 class UwConfig(C.Structure):
@@ -41,6 +42,7 @@ SIGNATURES = {
     "uw_ctx_create": (C.c_int, [C.POINTER(UwConfig), C.POINTER(_vp), C.c_int, _vp, C.POINTER(_vp)]),
     "uw_ctx_destroy": (C.c_int, [_vp]),
     "uw_ctx_bytes": (_i64, [_vp]),
+    "uw_ctx_cross_cache": (C.c_int, [_vp, C.c_int]),
     "uw_mel": (C.c_int, [_vp, _vp, _i64, _vp, C.c_int, _vp, _vp]),
     "uw_encode": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp]),
     "uw_cross_kv": (C.c_int, [_vp, _vp, C.c_int, _vp]),
