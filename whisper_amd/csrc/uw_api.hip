@@ -582,6 +582,14 @@ size_t cross_kv_layer_bytes(const uw_ctx* c) { return (size_t)c->Bm * c->S * 2 *
 size_t cross_vt_layer_bytes(const uw_ctx* c) { return (size_t)c->Bm * c->d * c->Spad * c->es; }
 size_t self_kv_layer_bytes(const uw_ctx* c) { return (size_t)c->Bm * c->Tm * 2 * c->d * c->es; }
 
+// page i of the 8-bit cross cache is block i of the windows one behind the other; every window has S frames
+__global__ void cross8_tables_kernel(int32_t* __restrict__ table, int pages, int32_t* __restrict__ len, int windows, int S)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < pages) table[i] = i;
+    if (i < windows) len[i] = S;
+}
+
 uw_kv8_cache cross8_cache(const uw_ctx* c, size_t layer)
 {
     const size_t pages = (size_t)c->Bm * c->cross8_width, codes = pages * c->H * 64 * 64, scales = pages * c->H;
@@ -1024,15 +1032,12 @@ int uw_ctx_cross_cache(uw_ctx* c, int format)
     if (format >= 0 && !c->cross8_codes) {
         const int W = (c->S + 63) / 64;
         const size_t pages = (size_t)c->Bm * W, Ld = c->dec.size();
-        // the host's tables first: nothing of the context changes before all of it is there
-        std::vector<int32_t> table(pages), len(c->Bm, c->S);
-        for (size_t i = 0; i < pages; ++i) table[i] = (int32_t)i;
         ALLOC(c->cross8_scales, Ld * 2 * pages * c->H * 4, true);
         ALLOC(c->cross8_table, pages * 4, false);
         ALLOC(c->cross8_len, (size_t)c->Bm * 4, false);
         ALLOC(c->cross8_pos, (size_t)c->Bm * 4, true);
-        UW_HIP_CHECK(hipMemcpy(c->cross8_table, table.data(), pages * 4, hipMemcpyHostToDevice));
-        UW_HIP_CHECK(hipMemcpy(c->cross8_len, len.data(), (size_t)c->Bm * 4, hipMemcpyHostToDevice));
+        hipLaunchKernelGGL(cross8_tables_kernel, dim3(ceil_div(pages, 256)), dim3(256), 0, nullptr, c->cross8_table, (int)pages, c->cross8_len, c->Bm, c->S);
+        UW_LAUNCH_CHECK();
         c->cross8_width = W;
         ALLOC(c->cross8_codes, Ld * 2 * pages * c->H * 64 * 64, true);
         UW_HIP_CHECK(hipDeviceSynchronize());

@@ -42,7 +42,7 @@ struct AttnArgs {
     int H, G, causal;
     int n_split;         // 1: an item is a row tile of a sequence; else at most so many items share a tile, each with a part of the keys
     int target, min_chunk;   // n_split > 1: items a head should come to, and the fewest blocks of 64 keys of one
-    int tiles, groups;   // row tiles per sequence (uniform), items of a head
+    int tiles;           // row tiles per sequence (uniform)
     int max_blocks;      // blocks that the table can hold, and one more: a longer sequence sees a page that does not exist
     int lds_rows;        // rows of a tile that can be in use
     float scale2;        // |scale| * log2(e)
@@ -188,8 +188,11 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
     float factor, lse;
     result_of(a, factor, lse);
     T* out = (T*)p.o.data + (p.ts.tok_start ? rg * p.o.sT : (long)b * p.o.sB + (long)t * p.o.sT) + (long)h * p.o.sH + d;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 v;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = from_f32<T>(acc[k] * factor);
+    for (int k = 0; k < 4; ++k) v[k] = from_f32<T>(acc[k] * factor);
+    *(T4*)out = v;
     if (p.lse && d == 0) p.lse[rg * p.H + h] = lse;
 }
 
@@ -689,7 +692,7 @@ constexpr int max_row_tiles(size_t elem, int D) { return elem == 4 && D == 128 ?
 struct AttnPlan {
     int rt, wk, wr;      // row tiles of 16 per wave, waves sharing keys, waves side by side on rows
     int n_split, target, min_chunk, tiles, max_blocks, lds_rows;
-    long groups, ws_bytes;
+    long groups, ws_bytes;   // items of a head
 };
 
 // How a call is cut.
@@ -700,7 +703,8 @@ struct AttnPlan {
 //    5000 keys 168 / 240.  Of the latter, tiles of 16 rows where a row is short (64 channels: 16 against 18 us, 32 against 36), of 32
 //    where keys are many bytes (2048 rows over 8192 keys of 128 channels: 184 against 107 us)
 //  - long sequences are cut further where the waves share the keys, into items of equal size (chunk_of), joined by a second launch.
-//    Short ones are not: up to 32 blocks, eight or four waves are through sooner than a second launch is
+//    Short ones are not: up to 32 blocks, eight or four waves are through sooner than a second launch is.  Nor are many: 512 tables of
+//    up to 64 blocks, or 4096 of any length, fill the chip evenly enough as they are
 AttnPlan plan_attention(const uw_kv8_attention_args* a)
 {
     AttnPlan p;
@@ -726,7 +730,7 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     const long alone = p.groups * c->n_kv_heads;             // workgroups without a cut
     p.n_split = 1;
     p.target = p.min_chunk = 0;
-    if (p.wk == 4 && p.max_blocks > 33 && !(alone >= 512 && p.max_blocks <= 65)) {
+    if (p.wk == 4 && p.max_blocks > 33 && !(alone >= 512 && p.max_blocks <= 65) && alone < 4096) {
         p.min_chunk = 8;
         // a tile's last item is a short one: they are counted in, so that all items find a place at once
         const long items = ceil_div(512, c->n_kv_heads);
@@ -800,7 +804,6 @@ int uw_kv8_cross_decode(int dtype, const Kv8StepParams& p, hipStream_t s)
     a.G = 1;
     a.n_split = 1;
     a.tiles = 1;
-    a.groups = p.B;
     a.lds_rows = 1;
     a.scale2 = LOG2E;                 // queries come scaled
     a.step.active = p.active;
@@ -858,7 +861,6 @@ int uw_kv8_attention(const uw_kv8_attention_args* a, void* stream)
     x.min_chunk = pl.min_chunk;
     x.max_blocks = pl.max_blocks;
     x.tiles = pl.tiles;
-    x.groups = (int)pl.groups;
     x.lds_rows = pl.lds_rows;
     x.scale2 = fabsf(a->scale) * LOG2E;
     x.neg = a->scale < 0.f ? 0x80000000u : 0u;

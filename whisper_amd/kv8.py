@@ -189,7 +189,7 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
     lib = L.load()
     head = (table.data_ptr(), kv_len.data_ptr(), tok_start.data_ptr() if packed else 0, n, width, B, T, _DTYPES[q.dtype], *cq,
             out.data_ptr(), T * heads * d, heads * d, d, lse.data_ptr() if return_lse else 0)
-    tail = (heads, 1 if causal else 0, d ** -0.5 if scale is None else scale, 0)
+    tail = (heads, 1 if causal else 0, d ** -0.5 if scale is None else float(scale), 0)
     args = cache._c + _ATTEND.pack(*head, 0, 0, *tail)
     need = lib.uw_kv8_attention_workspace_bytes(args)
     if need > 0:
