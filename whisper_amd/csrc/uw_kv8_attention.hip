@@ -309,39 +309,50 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     // blocks of 64 keys of this item, dealt to the waves
     const int blocks = min((lim_max >> 6) + ((lim_max & 63) ? 1 : 0), p.max_blocks);
     const int blk0 = split * chunk, blk1 = splits > 1 ? min(blocks, blk0 + chunk) : blocks;
-    const long page_bytes = (long)c.P * D;
     const int k_group = 16 * (rr >> 2), k_in = rr & 3;     // 16-key group and place in it of this lane's K rows
     int blk = blk0 + wk;
 
-    // 64 pages from the one of block `blk` on, one to a lane: id and scales, so that a step asks memory for nothing but codes
-    int win = 0, w_id = -1;
-    float w_ks = 0.f, w_vs = 0.f;
+    // 64 pages from the one of block `blk` on, one to a lane: where its codes begin, its K scale and the logarithm of its V scale, so that a
+    // step asks memory for nothing but codes and multiplies no addresses.  A page that does not exist is read as page 0 with NaN scales;
+    // a block of zeros (scale 0) has codes of zero, any scale does.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
+    int win = 0, w_lo = 0, w_hi = 0;
+    float w_ks = 0.f, w_lv = 0.f;
     auto window = [&](int from) {
         win = (from << 6) >> c.log2P;
-        w_id = kv8_page(c, b, (long)win + lane);
-        w_ks = w_vs = __uint_as_float(0x7fc00000u);
-        if (w_id >= 0) {
-            w_ks = c.ks[(long)w_id * c.Hkv + kvh] * p.scale2;
-            w_vs = c.vs[(long)w_id * c.Hkv + kvh];
+        const int id = kv8_page(c, b, (long)win + lane);
+        const long at = (long)max(id, 0) * c.Hkv + kvh, off = at * c.P * D;
+        w_lo = (int)off;
+        w_hi = (int)(off >> 32);
+        w_ks = w_lv = __uint_as_float(0x7fc00000u);
+        if (id >= 0) {
+            const float vs = c.vs[at];
+            w_ks = c.ks[at] * p.scale2;
+            w_lv = __builtin_amdgcn_logf(vs == 0.f ? 1.f : vs);
         }
     };
     // whether the pages of block x are in it
     auto in_window = [&](int x) { return (((x << 6) + 48) >> c.log2P) - win < 64; };
     // lane of the window that holds key j's page
     auto at_key = [&](int j) { return (j >> c.log2P) - win; };
+    auto page_at = [&](int j) {
+        const int w = at_key(j);
+        return (long)((unsigned long)(unsigned)__shfl(w_lo, w, 64) | (unsigned long)(unsigned)__shfl(w_hi, w, 64) << 32);
+    };
+    const bool whole = c.P >= 64;                          // a block lies in one page: K and V lanes look up the same
+    const int v_row = (SHARE ? wr * 16 + rr : rr) * c.P, k_row = (SHARE ? 4 * wr + k_in : k_in) * D + g4 * 16;
 
     uint4 kf[4][HALF], vf[D / 16];
     auto load_k = [&](int x) {
-        const int j = (x << 6) + k_group, id = max(0, __shfl(w_id, at_key(j), 64));
-        const uint8_t* kp = c.k + ((long)id * c.Hkv + kvh) * page_bytes + ((j & (c.P - 1)) + k_in) * D + g4 * 16;
+        const int j = (x << 6) + k_group;
+        const uint8_t* kp = c.k + page_at(j) + ((j & (c.P - 1)) * D + k_row);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = ld_codes<(WR == 1)>(kp + t * 4 * D + hf * 64);
     };
     auto load_v = [&](int x) {
-        const int j = (x << 6) + 16 * g4, id = max(0, __shfl(w_id, at_key(j), 64));
-        const uint8_t* vp = c.v + ((long)id * c.Hkv + kvh) * page_bytes + rr * c.P + (j & (c.P - 1));
+        const int j = (x << 6) + 16 * g4;
+        const uint8_t* vp = c.v + page_at(j) + ((j & (c.P - 1)) + v_row);
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(WR == 1)>(vp + d * 16 * c.P);
     };
@@ -355,9 +366,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     uint4 raw[2 * HALF];
     auto bring = [&](int x) {
         const int jk = (x << 6) + k_group, jv = (x << 6) + 16 * g4;
-        const int ik = max(0, __shfl(w_id, at_key(jk), 64)), iv = max(0, __shfl(w_id, at_key(jv), 64));
-        const uint8_t* kp = c.k + ((long)ik * c.Hkv + kvh) * page_bytes + ((jk & (c.P - 1)) + k_in + 4 * wr) * D + g4 * 16;
-        const uint8_t* vp = c.v + ((long)iv * c.Hkv + kvh) * page_bytes + (wr * 16 + rr) * c.P + (jv & (c.P - 1));
+        const long pk = page_at(jk), pv = whole ? pk : page_at(jv);
+        const uint8_t *kp = c.k + pk + ((jk & (c.P - 1)) * D + k_row), *vp = c.v + pv + ((jv & (c.P - 1)) + v_row);
 #pragma unroll
         for (int hf = 0; hf < HALF; ++hf) {
             raw[hf] = ld_codes<false>(kp + hf * 64);
@@ -389,7 +399,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         constexpr bool mask = decltype(masked)::value;
         const int j0 = blk << 6, jv = j0 + 16 * g4;
         const bool more = !SHARE && blk + WK < blk1;
-        const float kscale = __shfl(w_ks, at_key(jv), 64), vs = __shfl(w_vs, at_key(jv), 64);
+        const float kscale = __shfl(w_ks, at_key(jv), 64), lv = __shfl(w_lv, at_key(jv), 64);
         if (more && !in_window(blk + WK)) window(blk + WK);
         const int from = (blk & 1) * BUFFER + lane;      // SHARE
 
@@ -424,8 +434,6 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        // a block of zeros (scale 0) has codes of zero: any scale does.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
-        const float lv = __builtin_amdgcn_logf(vs == 0.f ? 1.f : vs);
         vtype pf[RT][2][NP];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
