@@ -10,7 +10,7 @@
 // exponentials of every chunk of every row -- the one pass over all scores, bound by HBM; (2) each chunk's workgroup joins the
 // rows' statistics, decides how many tokens stand, and sums the weights of its chunk of the one row that is drawn from (which is
 // in L2 or the Infinity Cache by then); (3) a workgroup per sequence finds the chunk, then the token in it.  Probabilities need no
-// (1); greedy verification needs the arg-max of (1) and then one small launch.
+// (1), logits without a draft no (2); greedy verification needs the arg-max of (1) and then one small launch.
 #include "../../include/uw_hip.h"
 #include "uw_common.h"
 #include "uw_kernels.h"
@@ -173,28 +173,23 @@ __device__ __forceinline__ double probability(const VerifyParams& p, float x, fl
     return p.probs ? (double)x : exp_neg(((double)x - (double)m) * p.inv_t) * r;
 }
 
-// (2) grid (chunks, B)
-template <typename T>
-__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
+// How many of a sequence's tokens stand, and the rows that the next one is drawn from: by all 256 threads, the same in all of them.
+// Eight positions at a time, 16 lanes to a row -- even slots the target's rows, odd ones the draft's -- so that all their statistics
+// are on their way at once.
+struct DecideScratch { double r[16], p[16]; float m[16], u[8]; };       // of a batch of rows: 1 / sum, probability of the drafted token
+template <typename T> __device__ __forceinline__ Chosen decide(const VerifyParams& p, int b, DecideScratch& s)
 {
-    __shared__ double s_r[16], s_p[16], s_z[4], s_w[4];        // of a batch of rows: 1 / sum, probability of the drafted token
-    __shared__ float s_m[16], s_u[8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x % p.chunks, b = blockIdx.x / p.chunks;
-    const int n = p.n_of(b), V = p.V;
+    const int tid = threadIdx.x, n = p.n_of(b);
     const T* tb = (const T*)p.target + (long)b * p.t_sB;
     const T* db = p.draft ? (const T*)p.draft + (long)b * p.d_sB : nullptr;
     const int32_t* d = p.drafted + (long)b * p.N;
-    const float* u = p.u + (long)b * (p.N + 1);
-
-    // How many tokens stand.  Eight positions at a time, 16 lanes to a row: even slots the target's rows, odd ones the draft's, so that
-    // all their statistics are on their way at once.
     int acc;
     for (int i0 = 0;; i0 += 8) {
         const int slot = tid >> 4, i = i0 + (slot >> 1);
         const bool is_draft = slot & 1;
         if (i <= n && (!is_draft || (db && i < n))) {
             const int di = i < n ? d[i] : -1;
-            const bool token = di >= 0 && di < V;
+            const bool token = di >= 0 && di < p.V;
             const float x = !token ? 0.f : is_draft ? to_f32<T>(db[(long)i * p.d_sN + di]) : to_f32<T>(tb[(long)i * p.t_sN + di]);
             float m = 0;
             double z = 1;
@@ -204,27 +199,35 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
             }
             const double r = 1.0 / z;
             if ((tid & 15) == 0) {
-                if (!is_draft) s_u[slot >> 1] = i < n ? u[i] : 0.f;
-                s_m[slot] = m;
-                s_r[slot] = r;
-                s_p[slot] = !token ? 0.0 : probability(p, x, m, r);       // an id outside the vocabulary is never accepted
+                if (!is_draft) s.u[slot >> 1] = i < n ? p.u[(long)b * (p.N + 1) + i] : 0.f;
+                s.m[slot] = m;
+                s.r[slot] = r;
+                s.p[slot] = !token ? 0.0 : probability(p, x, m, r);       // an id outside the vocabulary is never accepted
             }
         }
         __syncthreads();
         int run = 0;
-        while (run < 8 && i0 + run < n && (double)s_u[run] * (db ? s_p[2 * run + 1] : 1.0) < s_p[2 * run]) ++run;
+        while (run < 8 && i0 + run < n && (double)s.u[run] * (db ? s.p[2 * run + 1] : 1.0) < s.p[2 * run]) ++run;
         acc = i0 + run;
         if (run < 8) break;
         __syncthreads();
     }
+    const bool residual = db && acc < n, point = !db && acc < n && d[acc] >= 0 && d[acc] < p.V;
+    const int at = (acc & 7) * 2;
+    return Chosen{s.r[at], residual ? s.r[at + 1] : 1.0, s.m[at], residual ? s.m[at + 1] : 0.f, acc, residual ? 1 : point ? 2 : 0};
+}
 
-    // the rows that the next token is drawn from
-    const T* row = tb + (long)acc * p.t_sN;
-    const T* qrow = (db && acc < n) ? db + (long)acc * p.d_sN : nullptr;
-    const int point = (!db && acc < n && d[acc] >= 0 && d[acc] < V) ? d[acc] : -1, at_slot = (acc & 7) * 2;
-    const float mp = s_m[at_slot], mq = qrow ? s_m[at_slot + 1] : 0.f;
-    const double rp = s_r[at_slot], rq = qrow ? s_r[at_slot + 1] : 1.0;
-
+// (2) grid (chunks, B)
+template <typename T>
+__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
+{
+    __shared__ DecideScratch scratch;
+    __shared__ double s_z[4], s_w[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x % p.chunks, b = blockIdx.x / p.chunks, V = p.V;
+    const Chosen ch = decide<T>(p, b, scratch);
+    const T* row = (const T*)p.target + (long)b * p.t_sB + (long)ch.acc * p.t_sN;
+    const T* qrow = ch.mode == 1 ? (const T*)p.draft + (long)b * p.d_sB + (long)ch.acc * p.d_sN : nullptr;
+    const int point = ch.mode == 2 ? p.drafted[(long)b * p.N + ch.acc] : -1;
     float x[PER], y[PER];
     const int j0 = c * CHUNK;
     const float none = p.probs ? 0.f : -INFINITY;
@@ -233,10 +236,10 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
     double sp = 0, sr = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-        const double w = probability(p, x[k], mp, rp);
+        const double w = probability(p, x[k], ch.mp, ch.rp);
         sp += w;
         if (qrow) {
-            const double r = w - probability(p, y[k], mq, rq);
+            const double r = w - probability(p, y[k], ch.mq, ch.rq);
             sr += r != r ? r : fmax(r, 0.0);
         } else if (score_index<T>(j0, k) != point) {
             sr += w;
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyParams p)
         double* at = p.mass + ((long)b * p.chunks + c) * 2;
         at[0] = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
         at[1] = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
-        if (c == 0) p.chosen[b] = Chosen{rp, rq, mp, mq, acc, qrow ? 1 : point >= 0 ? 2 : 0};
+        if (c == 0) p.chosen[b] = ch;
     }
 }
 
@@ -262,19 +265,47 @@ __device__ __forceinline__ void write_tokens(const VerifyParams& p, int b, int a
         p.tokens[(long)b * (p.N + 1) + i] = i < acc ? p.drafted[(long)b * p.N + i] : i == acc ? next : -1;
 }
 
-// (3) grid B: which chunk, then which token
-template <typename T>
+// (3) grid B: which chunk, then which token.  OWN: logits without a draft -- the chunks' sums of (1) are their masses but for the one that
+// loses the drafted token, so (2) is not needed.
+template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
 {
-    __shared__ double s_c[256];
+    __shared__ DecideScratch scratch;
+    __shared__ double s_c[8];
     __shared__ double s_r;
     __shared__ int s_chunk, s_next, s_last[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
-    const Chosen ch = p.chosen[b];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x, V = p.V;
+    const Chosen ch = OWN ? decide<T>(p, b, scratch) : p.chosen[b];
     const double* mass = p.mass + (long)b * p.chunks * 2;
-    // totals of the residual and of p: a thread a chunk, added up wave by wave in a fixed order
+    const ChunkStat* st = p.t_stat + ((long)b * (p.N + 1) + ch.acc) * p.chunks;
+    const T* row = (const T*)p.target + (long)b * p.t_sB + (long)ch.acc * p.t_sN;
+    const T* qrow = (const T*)p.draft + (long)b * p.d_sB + (long)ch.acc * p.d_sN;
+    const int point = ch.mode == 2 ? p.drafted[(long)b * p.N + ch.acc] : -1;
+
+    double without = 0;                       // OWN: mass of the drafted token's chunk without it
+    if (OWN && ch.mode == 2) {
+        float x[PER];
+        const int j0 = point / CHUNK * CHUNK;
+        load_scores<T>(row, j0, V, x, -INFINITY);
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (score_index<T>(j0, k) != point) without += probability(p, x[k], ch.mp, ch.rp);
+        without = wave_sum_d(without);
+        if (lane == 0) s_c[wave] = without;
+        __syncthreads();
+        without = (s_c[0] + s_c[1]) + (s_c[2] + s_c[3]);
+        __syncthreads();
+    }
+    // of the residual (0) or of p (1)
+    auto mass_of = [&](int c, int which) {
+        if constexpr (!OWN) return mass[2 * c + which];
+        if (which == 0 && ch.mode == 2 && c == point / CHUNK) return without;
+        const ChunkStat s = st[c];
+        return (s.mx == -INFINITY ? s.z : s.z * exp_neg(((double)s.mx - (double)ch.mp) * p.inv_t)) * ch.rp;
+    };
+    // totals: a thread a chunk, added up wave by wave in a fixed order
     double own[2] = {0, 0};
-    for (int c = tid; c < p.chunks; c += 256) { own[0] += mass[2 * c]; own[1] += mass[2 * c + 1]; }
+    for (int c = tid; c < p.chunks; c += 256) { own[0] += mass_of(c, 0); own[1] += mass_of(c, 1); }
     own[0] = wave_sum_d(own[0]);
     own[1] = wave_sum_d(own[1]);
     if (lane == 0) { s_c[wave] = own[0]; s_c[4 + wave] = own[1]; }
@@ -290,7 +321,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
         double cum = 0, before = 0, last_before = 0;
         int at = -1, last = 0;
         for (int c0 = 0; c0 < p.chunks && at < 0; c0 += 64) {
-            const double w = c0 + lane < p.chunks ? mass[2 * (c0 + lane) + which] : 0.0;
+            const double w = c0 + lane < p.chunks ? mass_of(c0 + lane, which) : 0.0;
             for (int k = 0; k < min(64, p.chunks - c0); ++k) {
                 const double wk = __shfl(w, k, 64);
                 if (wk > 0) { last = c0 + k; last_before = cum; }
@@ -305,10 +336,8 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
         }
     }
     __syncthreads();
-    const int j0 = s_chunk * CHUNK, V = p.V, b0 = j0 + tid * PER;
-    const T* row = (const T*)p.target + (long)b * p.t_sB + (long)ch.acc * p.t_sN;
-    const T* qrow = (const T*)p.draft + (long)b * p.d_sB + (long)ch.acc * p.d_sN;
-    const int mode = which ? 0 : ch.mode, point = mode == 2 ? p.drafted[(long)b * p.N + ch.acc] : -1;
+    const int j0 = s_chunk * CHUNK, b0 = j0 + tid * PER;
+    const int mode = which ? 0 : ch.mode;
     // a thread's 16 scores follow one another here, so that its weights can be added up in order
     constexpr int VEC = Piece<T>::VEC;
     auto run_of = [&](const T* from, float* x) {
@@ -332,7 +361,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
     for (int k = 0; k < PER; ++k) {
         double v = probability(p, x[k], ch.mp, ch.rp);
         if (mode == 1) v = fmax(v - probability(p, y[k], ch.mq, ch.rq), 0.0);
-        if (b0 + k == point) v = 0;
+        if (mode == 2 && b0 + k == point) v = 0;
         w[k] = v;
         sum += v;
     }
@@ -473,12 +502,16 @@ int uw_verify_draft(const uw_verify_args* a, void* stream)
             if (f32) hipLaunchKernelGGL((verify_rows_kernel<float, false>), rows, one, 0, s, p);
             else hipLaunchKernelGGL((verify_rows_kernel<bf16_t, false>), rows, one, 0, s, p);
         }
-        if (f32) {
+        const dim3 seqs(a->B);
+        if (!a->probs && !a->draft) {
+            if (f32) hipLaunchKernelGGL((verify_pick_kernel<float, true>), seqs, one, 0, s, p);
+            else hipLaunchKernelGGL((verify_pick_kernel<bf16_t, true>), seqs, one, 0, s, p);
+        } else if (f32) {
             hipLaunchKernelGGL(verify_mass_kernel<float>, mass, one, 0, s, p);
-            hipLaunchKernelGGL(verify_pick_kernel<float>, dim3(a->B), one, 0, s, p);
+            hipLaunchKernelGGL((verify_pick_kernel<float, false>), seqs, one, 0, s, p);
         } else {
             hipLaunchKernelGGL(verify_mass_kernel<bf16_t>, mass, one, 0, s, p);
-            hipLaunchKernelGGL(verify_pick_kernel<bf16_t>, dim3(a->B), one, 0, s, p);
+            hipLaunchKernelGGL((verify_pick_kernel<bf16_t, false>), seqs, one, 0, s, p);
         }
     }
     UW_LAUNCH_CHECK();
