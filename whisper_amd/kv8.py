@@ -5,6 +5,7 @@ A token takes half of its bf16 size, so decoding, which is bound by the stream o
 Calls run on the tensors' device and its current stream, do not synchronise and may be captured into a graph."""
 from __future__ import annotations
 
+from functools import lru_cache
 from struct import Struct
 from typing import Optional, Tuple
 
@@ -18,6 +19,8 @@ _DTYPES = {torch.float32: L.UW_DTYPE_F32, torch.bfloat16: L.UW_DTYPE_BF16}
 
 # the argument structures of the C ABI behind their uw_kv8_cache
 _CACHE = Struct("@4P6i")
+_CACHE_DIMS = Struct("@6i")
+_ADDRESSES = 32                                  # bytes of a uw_kv8_cache in front of its sizes
 _STORE = Struct("@3Pq4i P3q P3q")
 _ATTEND = Struct("@3Pq4i P3q P3q 2Pq2ifi")
 
@@ -161,6 +164,16 @@ def read(cache: KV8Cache, table: torch.Tensor, first: torch.Tensor, n_tok: int, 
     return k, v
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(dims: bytes, n: int, width: int, B: int, T: int, dtype: int, packed: bool, heads: int) -> int:
+    """Scratch of a call of these sizes (they alone decide: the addresses here are none)."""
+    need = L.load().uw_kv8_attention_workspace_bytes(_CACHE.pack(64, 64, 64, 64, *_CACHE_DIMS.unpack(dims)) + _ATTEND.pack(
+        64, 64, 64 if packed else 0, n, width, B, T, dtype, 64, 0, 0, 0, 64, 0, 0, 0, 0, 0, 0, heads, 0, 1.0, 0))
+    if need < 0:
+        L.check(1)
+    return (need + 15) // 16 * 16
+
+
 def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: torch.Tensor, tok_start: Optional[torch.Tensor] = None,
               causal: bool = True, scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
     """softmax(scale * q . K) V over the first kv_len[b] cached tokens of each sequence.  q [B, T, heads, head_dim], or
@@ -186,14 +199,11 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = cache.k_scale.new_empty(shape[:-1]) if return_lse else None
     n, T = (shape[0], 0) if packed else (B * shape[1], shape[1])
-    lib = L.load()
-    head = (table.data_ptr(), kv_len.data_ptr(), tok_start.data_ptr() if packed else 0, n, width, B, T, _DTYPES[q.dtype], *cq,
-            out.data_ptr(), T * heads * d, heads * d, d, lse.data_ptr() if return_lse else 0)
-    tail = (heads, 1 if causal else 0, d ** -0.5 if scale is None else float(scale), 0)
-    args = cache._c + _ATTEND.pack(*head, 0, 0, *tail)
-    need = lib.uw_kv8_attention_workspace_bytes(args)
-    if need > 0:
-        ws = cache.k_scale.new_empty((need + 3) // 4)
-        args = cache._c + _ATTEND.pack(*head, ws.data_ptr(), need, *tail)
-    _call(lib.uw_kv8_attention, args, dev)
+    dtype = _DTYPES[q.dtype]
+    need = _workspace_bytes(cache._c[_ADDRESSES:], n, width, B, T, dtype, packed, heads)
+    ws = cache.k_scale.new_empty(need // 4) if need else None
+    _call(L.load().uw_kv8_attention, cache._c + _ATTEND.pack(
+        table.data_ptr(), kv_len.data_ptr(), tok_start.data_ptr() if packed else 0, n, width, B, T, dtype, *cq, out.data_ptr(), T * heads * d,
+        heads * d, d, lse.data_ptr() if return_lse else 0, ws.data_ptr() if need else 0, need, heads, 1 if causal else 0,
+        d ** -0.5 if scale is None else float(scale), 0), dev)
     return (out, lse) if return_lse else out

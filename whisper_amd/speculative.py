@@ -3,6 +3,7 @@ uw_verify_draft in include/uw_hip.h).  The scores are what `Engine.decoder_forwa
 positions: one pass of the decoder scores all of them."""
 from __future__ import annotations
 
+from functools import lru_cache
 from struct import Struct
 from typing import Optional, Tuple
 
@@ -19,6 +20,16 @@ def _ints(x: torch.Tensor, shape, what: str, dev: int) -> torch.Tensor:
     if x.shape != shape or x.dtype not in (torch.int32, torch.int64) or x.get_device() != dev:
         raise ValueError(f"{what} must be int32 {list(shape)} beside target, got {x.dtype} {tuple(x.shape)} on {x.device}")
     return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(dtype: int, B: int, N: int, V: int, greedy: bool, probs: bool, with_draft: bool) -> int:
+    """Scratch of a call of these sizes (they alone decide: the addresses here are none)."""
+    need = L.load().uw_verify_draft_workspace_bytes(_ARGS.pack(64, 0, 0, 64 if with_draft else 0, 0, 0, 64, 0, 64, 64, 64, 0, 0, dtype, B, N, V,
+                                                               0.0 if greedy else 1.0, 1 if probs else 0))
+    if need < 0:
+        L.check(1)
+    return (need + 15) // 16 * 16
 
 
 def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: Optional[torch.Tensor] = None,
@@ -65,16 +76,15 @@ def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: Optional
         target = target.contiguous()
         st = target.stride()
     accepted, tokens = drafted.new_empty(B), drafted.new_empty((B, N + 1))
-    lib = L.load()
-    use_draft = draft is not None and not greedy
-    head = (target.data_ptr(), st[0], st[1], draft.data_ptr() if use_draft else 0, *(draft.stride()[:2] if use_draft else (0, 0)),
-            drafted.data_ptr(), 0 if n_drafted is None else n_drafted.data_ptr(), 0 if greedy else uniforms.data_ptr(), accepted.data_ptr(),
-            tokens.data_ptr())
-    tail = (_DTYPES[target.dtype], B, N, V, temperature, 1 if probs else 0)
-    args = _ARGS.pack(*head, 0, 0, *tail)
-    need = lib.uw_verify_draft_workspace_bytes(args)
-    if need > 0:
-        ws = drafted.new_empty((need + 3) // 4)
-        args = _ARGS.pack(*head, ws.data_ptr(), need, *tail)
-    _call(lib.uw_verify_draft, args, dev)
+    if draft is None or greedy:
+        at, dB, dN = 0, 0, 0
+    else:
+        at, (dB, dN, _) = draft.data_ptr(), draft.stride()
+    dtype = _DTYPES[target.dtype]
+    need = _workspace_bytes(dtype, B, N, V, greedy, probs, at != 0)
+    ws = drafted.new_empty(need // 4)
+    _call(L.load().uw_verify_draft, _ARGS.pack(
+        target.data_ptr(), st[0], st[1], at, dB, dN, drafted.data_ptr(), 0 if n_drafted is None else n_drafted.data_ptr(),
+        0 if greedy else uniforms.data_ptr(), accepted.data_ptr(), tokens.data_ptr(), ws.data_ptr(), need, dtype, B, N, V, temperature,
+        1 if probs else 0), dev)
     return accepted, tokens
