@@ -16,7 +16,7 @@ namespace {
 // so neither K nor V nor P passes through LDS.  K scales multiply the scores, V scales ride in the exponent of the weights; one per 16
 // keys at least, so one per lane.  References, sums and outputs are f32.
 //
-// bf16 queries enter exactly.  Their weights are rounded once to f16 for P V -- 2^-12 of each, and 2^-25 of the largest where they run
+// bf16 queries enter exactly.  Their weights are rounded once to f16 for P V -- 2^-11 of each at most, and 2^-25 of the largest where they run
 // out of exponent -- an eighth of what the bf16 result is rounded by; the codes are exact in f16 too.  f32 queries and weights enter as
 // three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.
 // What a decoder step adds: one query token per window, its output in the operand layout of the product that follows, and the
@@ -705,11 +705,14 @@ struct AttnPlan {
 
 // How a call is cut.
 //  - up to 16 rows of a kv head: one row tile, the waves share the keys
-//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), if that gives 384 workgroups; else tiles of 16 or 32
-//    rows whose four waves share the keys -- more workgroups for the same rows.  Measured (us, side by side / sharing keys): 170 rows x
-//    64 heads over 1500 keys 32 / 18, 2000 rows x 8 heads 38 / 17, 170 rows x 192 heads 45 / 46, the 33380 rows of 12 heads over
-//    5000 keys 168 / 240.  Of the latter, tiles of 16 rows where a row is short (64 channels: 16 against 18 us, 32 against 36), of 32
-//    where keys are many bytes (2048 rows over 8192 keys of 128 channels: 184 against 107 us)
+//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), where that gives a workgroup to each of the 256 CUs,
+//    with 64 channels to one and a half times as many; else tiles of 16 or 32 rows whose four waves share the keys -- more workgroups
+//    for the same rows.  Measured (us, side by side / tiles of 32 / tiles of 16; bf16, workgroups of the first): 64 channels, 170 rows
+//    over 1500 keys: 128: 31.0 / 21.2 / 20.7, 256: 31.1 / 27.7 / 32.2, 384: 42.2 / 44.7 / 56.3, 512: 42.9 / 58.8 / 74.5; 2048 causal rows
+//    over 4096 keys: 256: 74.1 / 68.2 / 91.5, 384: 95.2 / 97.5 / 127; 33380 causal rows of 4 heads over 5000 keys 151 / 225 / 296.
+//    128 channels, 2048 causal rows over 8192 keys: 128: 198 / 122 / 211, 192: 199 / 184 / 325, 256: 199 / 242 / 445.
+//    Tiles of 16 where 64-channel rows are few, 12800 of all heads, or f32: 10880 rows over 1500 keys 20.4 / 21.2 (32 rows), 16320 29.0 /
+//    26.5, 2720 10.3 / 14.7; f32 10880 32.0 / 36.1, 19040 43.6 / 48.0.  (Rows of 128 channels make too little of a key's many bytes.)
 //  - long sequences are cut further where the waves share the keys, into items of equal size (chunk_of), joined by a second launch.
 //    Short ones are not: up to 32 blocks, eight or four waves are through sooner than a second launch is.  Nor are many: 512 tables of
 //    up to 64 blocks, or 4096 of any length, fill the chip evenly enough as they are
@@ -725,10 +728,11 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     p.wk = 4;
     p.wr = 1;
     if (rows > 32) {
-        if ((long)ceil_div(rows, 64 * p.rt) * B * c->n_kv_heads >= 384) {
+        const long heads = (long)B * c->n_kv_heads;
+        if (ceil_div(rows, 64 * p.rt) * heads >= (c->head_dim == 64 ? 384 : 256)) {
             p.wk = 1;
             p.wr = 4;
-        } else if (c->head_dim == 64) {
+        } else if (c->head_dim == 64 && (a->seqs.dtype == UW_DTYPE_F32 || rows * heads < 12800)) {
             p.rt = 1;
         }
     }
