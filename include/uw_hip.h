@@ -176,8 +176,8 @@ int uw_profile_span(uw_ctx* ctx, int kind, int64_t* launches_total, int64_t* lau
  * Formats: UW_KV8_INT8 (codes -127..127) and UW_KV8_E4M3 (1-4-3 without infinities, scales are powers of two).  page: 16, 32,
  * 64, 128 or 256; head_dim: 64 or 128.  k and v must be 16-byte aligned.
  * table i32 [B][table_width]: the page of each block of a sequence, block i holding positions i * page ... Entries behind a
- * sequence's end are not read.  A page id outside 0..n_pages-1, or a position behind the table, is never accessed: an append
- * skips it, a read and an attention row that sees it give NaN.
+ * sequence's end are not read.  A page id outside 0..n_pages-1, or a position before 0 or behind the table, is never accessed:
+ * an append skips it, a read and an attention row that sees it give NaN.
  * Tokens come either T per sequence (tok_start NULL, T > 0, n_tok = B * T), sequence b's first row at b * seq_stride, or packed
  * one sequence behind the other (tok_start i32 [B+1], row r at r * tok_stride; T and seq_stride are ignored); rows behind
  * tok_start[B] are neither read nor written.  Strides are in elements; element (row, head, i) lies at row + head * head_stride + i;
@@ -228,7 +228,7 @@ int uw_kv8_read(const uw_kv8_store_args* args, void* stream);
 /* Attention of n_heads query heads (a multiple of n_kv_heads; query head h reads kv head h / (n_heads / n_kv_heads)) over the
  * first len[b] cached tokens; with causal != 0 token t of the n tokens of a sequence sees keys 0 .. len[b] - n + t (its own
  * key, appended before, is the last).  o: rows like q; lse (may be NULL) f32 [n_tok][n_heads]: log of the sum of exp(scores).
- * A row that sees no key gives 0 and lse = -inf.  scale multiplies q.k.  ws: ws_bytes of scratch, at least what
+ * A row that sees no key (len[b] <= 0 among others) gives 0 and lse = -inf.  scale multiplies q.k.  ws: ws_bytes of scratch, at least what
  * uw_kv8_attention_workspace_bytes() answers for the same arguments (it reads no device memory; -1: arguments refused),
  * 16-byte aligned, not shared by calls that may run at the same time; NULL if that is 0. */
 int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_attention_args* args);

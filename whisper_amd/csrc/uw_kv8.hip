@@ -6,10 +6,10 @@
 
 namespace {
 
-// blocks that n tokens from position pos on touch
+// blocks that n tokens from position pos on touch (positions before the first lie in blocks before the first, which have no page)
 __device__ __forceinline__ int touched(int pos, int n, int log2P)
 {
-    return (n <= 0 || pos < 0) ? 0 : (int)((((unsigned)pos + (unsigned)n - 1) >> log2P) - ((unsigned)pos >> log2P) + 1);
+    return n <= 0 ? 0 : (int)(((unsigned)(pos & ((1 << log2P) - 1)) + (unsigned)n - 1) >> log2P) + 1;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -36,11 +36,10 @@ __device__ __forceinline__ bool find_block(const Kv8View& c, const TokSpan& ts, 
         if (j >= touched(pos_of[o.b], ts.T, c.log2P)) return false;
     }
     const int pos = pos_of[o.b], n = ts.count(o.b);
-    const long blk = (pos >> c.log2P) + j, p0 = blk << c.log2P;      // first position of the block
-    const int t0 = (int)max(0l, p0 - pos), t1 = (int)min((long)n, p0 + c.P - pos);
-    o.blk = blk;
-    o.r0 = (int)(pos + t0 - p0);
-    o.rows = t1 - t0;
+    const int in = pos & (c.P - 1), t0 = max(0, (j << c.log2P) - in);      // place in its block of the first token; the call's first token in block j
+    o.blk = (long)(pos >> c.log2P) + j;
+    o.r0 = j ? 0 : in;
+    o.rows = min(n - t0, c.P - o.r0);
     o.row = ts.tok_start ? (ts.first(o.b) + t0) * a.sT : (long)o.b * a.sB + (long)t0 * a.sT;
     return true;
 }

@@ -166,10 +166,13 @@ __device__ __forceinline__ float across_groups_max(float x)
 // what a wave, a workgroup or an item knows of a row beside its output
 struct RowState { float m, l, ms; };
 
-__device__ __forceinline__ void result_of(const RowState& a, float& factor, float& lse)
+// out = o * f0 * f1, f0 f1 = 2^(m - ms) / l in two steps: one alone runs out of exponent where all values are very small.  A row that saw
+// no key has l = 0
+__device__ __forceinline__ void result_of(const RowState& a, float& f0, float& f1, float& lse)
 {
-    // out = o 2^(m - ms) / l; a row that saw no key has l = 0
-    factor = a.l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a.m - a.ms) / a.l;
+    f1 = __builtin_amdgcn_exp2f(0.5f * (a.m - a.ms));
+    f0 = a.l == 0.f ? 0.f : f1 / a.l;
+    if (a.l == 0.f) f1 = 0.f;
     lse = a.l == 0.f ? -INFINITY : a.ms * LN2 + logf(a.l);
 }
 
@@ -185,13 +188,13 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
         if (d == 0) { at[D] = a.m; at[D + 1] = a.l; at[D + 2] = a.ms; }
         return;
     }
-    float factor, lse;
-    result_of(a, factor, lse);
+    float f0, f1, lse;
+    result_of(a, f0, f1, lse);
     T* out = (T*)p.o.data + (p.ts.tok_start ? rg * p.o.sT : (long)b * p.o.sB + (long)t * p.o.sT) + (long)h * p.o.sH + d;
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 v;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = from_f32<T>(acc[k] * factor);
+    for (int k = 0; k < 4; ++k) v[k] = from_f32<T>(acc[k] * f0 * f1);
     *(T4*)out = v;
     if (p.lse && d == 0) p.lse[rg * p.H + h] = lse;
 }
@@ -203,7 +206,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
 // whole 1 KiB pieces, without bank conflicts.  Two buffers and one barrier a block: while block x is worked on, x + 1 is converted
 // and the codes of x + 2 are under way in eight registers.
 template <int F, typename T, int D, int RT, int WK, int WR, bool STEP>
-__global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
+__global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : 3) : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
     constexpr bool SHARE = WR == 4;
@@ -449,10 +452,14 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
                 for (int t = 0; t < 4; ++t) *(f32x4*)(scores + jv + 4 * t) = st[i][t] * kscale;
             }
-            float x[16], sum, unit;
+            float x[16], sum, unit, lw = lv;
             auto weigh = [&](float base, float base_s) {
-                const float nb = lv - base;
-                unit = __builtin_amdgcn_exp2f((base - base_s) - lv);      // what the sum of x counts in l
+                // a V scale below 2^-64 of what the references stand for is taken as that: its weights would run out of exponent, and l
+                // lose them
+                const float least = (base - base_s) - 64.f;
+                lw = lv < least ? least : lv;                     // (a NaN stays)
+                const float nb = lw - base;
+                unit = __builtin_amdgcn_exp2f((base - base_s) - lw);      // what the sum of x counts in l
 #pragma unroll
                 for (int k = 0; k < 16; ++k) x[k] = __builtin_amdgcn_exp2f(fmaf(st[i][k >> 2][k & 3], kscale, nb));
                 if constexpr (mask) {                            // a scale behind the end may be NaN
@@ -469,7 +476,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             bool follow = true;
             if constexpr (!mask) {
                 weigh(m[i], ms[i]);
-                follow = __any(sum > 0x1p10f || sum * unit > 0x1p60f);
+                follow = __any(sum > 0x1p10f || sum * unit > 0x1p30f);
             }
             if (follow) {
                 if constexpr (!mask) asm volatile("");           // rare: nothing of it belongs in front of the branch
@@ -490,6 +497,12 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             }
             // (a poisoned scale of a block that is seen shows in the sum)
             if (!mask || left > 0) l[i] = fmaf(sum, unit, l[i]);
+            // (f16 has nothing below 2^-25: weights of a V scale that was raised, at most 2^(30 - 64), are 0 there in any case)
+            if (NP > 1 && lw > lv) {
+                const float down = __builtin_amdgcn_exp2f(lv - lw);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] *= down;
+            }
             if constexpr (NP == 1) {
 #pragma unroll
                 for (int k = 0; k < 16; ++k) pf[i][k >> 3][0][k & 7] = (_Float16)x[k];
@@ -601,11 +614,11 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                 for (int k = 0; k < 4; ++k) acc[k] += y[k] * f;
             }
             if constexpr (STEP) {
-                float factor, lse;
-                result_of(a, factor, lse);
+                float f0, f1, lse;
+                result_of(a, f0, f1, lse);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float v = acc[k] * factor;
+                    const float v = acc[k] * f0 * f1;
                     const T hi = from_f32<T>(v);
                     const long at = frag_elem_offset<T>(b, kvh * 64 + d + k, p.step.d);
                     ((T*)p.o.data)[at] = hi;
@@ -675,10 +688,10 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p, int tile_rows
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) acc[k] += x[k * 64 + lane] * f;
     }
-    float factor, lse;
-    result_of(a, factor, lse);
+    float f0, f1, lse;
+    result_of(a, f0, f1, lse);
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k) ((T*)p.o.data)[oat + (long)h * p.o.sH + k * 64 + lane] = from_f32<T>(acc[k] * factor);
+    for (int k = 0; k < D / 64; ++k) ((T*)p.o.data)[oat + (long)h * p.o.sH + k * 64 + lane] = from_f32<T>(acc[k] * f0 * f1);
     if (p.lse && lane == 0) p.lse[row * p.H + h] = lse;
 }
 
