@@ -18,7 +18,14 @@ namespace {
 //
 // bf16 queries enter exactly.  Their weights are rounded once to f16 for P V -- 2^-11 of each at most, and 2^-25 of the largest where they run
 // out of exponent -- an eighth of what the bf16 result is rounded by; the codes are exact in f16 too.  f32 queries and weights enter as
-// three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at the bf16 rate.
+// three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a third of the bf16 rate.
+//
+// What bounds it: few rows of a head -- the stream of codes; 128 windows' token over 1500 keys of 12 heads (296 MB) 48.8 us, 6.1 TB/s; five
+// tokens of 4 heads a kv head over long ragged tables (297 MB) 58.6 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
+// which has a multiply-add, an exponential (a quarter of the rate), an addition and half a conversion to do for each weight, beside the
+// 128 or 256 multiply-adds of the matrix unit: 33380 causal rows of 4 heads over 5000 keys 144 us, 750 TFLOP/s; of 128 channels 242 us,
+// 890.  One window -- a chain of lengths, pages, codes and the join of eight waves: 9.9 us.
+//
 // What a decoder step adds: one query token per window, its output in the operand layout of the product that follows, and the
 // probabilities of the alignment heads.
 struct StepArgs {
@@ -206,7 +213,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
 // whole 1 KiB pieces, without bank conflicts.  Two buffers and one barrier a block: while block x is worked on, x + 1 is converted
 // and the codes of x + 2 are under way in eight registers.
 template <int F, typename T, int D, int RT, int WK, int WR, bool STEP>
-__global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : 3) : RT * D * sizeof(T) <= 512 ? 2 : 1) void kv8_attention_kernel(AttnArgs p)
+__global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : 3) : 2) void kv8_attention_kernel(AttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
     constexpr bool SHARE = WR == 4;
@@ -222,7 +229,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 
     // which kv head, sequence, rows and part of the keys.  Heads run fastest: a head's workgroups land on one XCD when their number
     // is a multiple of 8, and share its L2.  The last rows of all sequences come first: causal ones see most, and a long item that
-    // starts late is waited for (4500, 2782 and 1063 rows: 197 us in the sequences' order, 171 so).
+    // starts late is waited for (4500, 2782 and 1063 tokens of 16 heads: 187 us in the sequences' order, 156 so).
     int b, tile, split = 0, splits = 1, chunk = 0;
     const int kvh = blockIdx.x % c.Hkv, item = blockIdx.x / c.Hkv;
     if (p.n_split > 1) {
@@ -646,7 +653,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     }
 }
 
-// joins the parts of a row whose keys were cut: a wave per (token, head)
+// joins the parts of a row whose keys were cut: a wave per (token, head), bound by the latency of lengths, references and parts one behind
+// the other (1280 rows of 128 channels 4.8 us)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p, int tile_rows)
 {

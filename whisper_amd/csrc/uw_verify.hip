@@ -11,6 +11,10 @@
 // rows' statistics, decides how many tokens stand, and sums the weights of its chunk of the one row that is drawn from (which is
 // in L2 or the Infinity Cache by then); (3) a workgroup per sequence finds the chunk, then the token in it.  Probabilities need no
 // (1), logits without a draft no (2); greedy verification needs the arg-max of (1) and then one small launch.
+//
+// Measured: 64 windows, up to five tokens, both models' f32 logits (V 51865, 146 MB if all are read) 27 + 16 + 9.5 us: (1) 5.4 TB/s, (2) and
+// (3) chains of statistics, decision, scores and sums, for which few rows are left to work side by side.  One window of four tokens 4.1 + 12 us.
+// Greedy, 128 windows of four tokens, bf16 (66 MB) 17.6 + 4.0 us.
 #include "../../include/uw_hip.h"
 #include "uw_common.h"
 #include "uw_kernels.h"
@@ -29,7 +33,7 @@ struct VerifyParams {
     const int32_t *drafted, *n_drafted;
     const float* u;
     int B, N, V, chunks;
-    double inv_t;
+    double per_t, least;            // log2(e) / temperature; the difference of scores that is 2^-1000
     int probs;
     int32_t *accepted, *tokens;
     ChunkStat *t_stat, *d_stat;     // [B][N + 1][chunks], [B][N][chunks]
@@ -39,27 +43,30 @@ struct VerifyParams {
     __device__ __forceinline__ int n_of(int b) const { return n_drafted ? min(max(n_drafted[b], 0), N) : N; }
 };
 
-// exp(t) for t <= 0 (and NaN): 2^n e^r, |r| <= ln2 / 2, e^r by its series to r^11 (next term 6e-15 relative).  A dozen f64
-// instructions, against the library's table and special cases.
-__device__ __forceinline__ double exp_neg(double t)
+// 2^t, t = d * per_t, for -1000 <= t <= 0: 2^n 2^r with n the nearest whole number (what t + 1.5 2^52 has in its last bits), |r| <= 1/2;
+// 2^r by the polynomial that meets it at the nine Chebyshev nodes of [-1/2, 1/2], 1.1e-12 off at most; n added to the exponent.  That
+// moves one draw in ten million across a border between two tokens (2e-5 apart on average); the uniform numbers come in steps of 6e-8.
+// Twelve f64 instructions; they are what these kernels wait for as much as for memory (with eighteen, 64 windows took 48 us, now 43).
+// A NaN stays one.
+__device__ __forceinline__ double pow2_near(double d, double per_t)
 {
-    t = t < -800.0 ? -800.0 : t;
-    const double n = rint(t * 1.4426950408889634074);
-    double r = fma(n, -0.6931471824645996, t);      // ln 2 as its float, n times which is exact, and the rest
-    r = fma(n, 1.904654299957768e-09, r);
-    double y = 1.0 / 39916800.0;
-    y = fma(y, r, 1.0 / 3628800.0);
-    y = fma(y, r, 1.0 / 362880.0);
-    y = fma(y, r, 1.0 / 40320.0);
-    y = fma(y, r, 1.0 / 5040.0);
-    y = fma(y, r, 1.0 / 720.0);
-    y = fma(y, r, 1.0 / 120.0);
-    y = fma(y, r, 1.0 / 24.0);
-    y = fma(y, r, 1.0 / 6.0);
-    y = fma(y, r, 0.5);
+    const double whole = 6755399441055744.0, s = fma(d, per_t, whole), r = fma(d, per_t, whole - s);
+    double y = 1.3255199372687166e-06;
+    y = fma(y, r, 1.5310079984429433e-05);
+    y = fma(y, r, 0.00015403455966378488);
+    y = fma(y, r, 0.0013333450565774538);
+    y = fma(y, r, 0.009618129159246654);
+    y = fma(y, r, 0.05550410941208298);
+    y = fma(y, r, 0.24022650695813655);
+    y = fma(y, r, 0.6931471805459328);
     y = fma(y, r, 1.0);
-    y = fma(y, r, 1.0);
-    return ldexp(y, (int)n);
+    return __hiloint2double(__double2hiint(y) + (__double2loint(s) << 20), __double2loint(y));
+}
+// the same for all d <= 0: 0 below 2^-1000, so that a score of -inf has no weight at all
+__device__ __forceinline__ double pow2_neg(double d, const VerifyParams& p)
+{
+    const double y = pow2_near(d, p.per_t);
+    return d < p.least ? 0.0 : y;
 }
 
 // PER scores of a chunk: piece u of thread t begins at u * 256 * VEC + t * VEC; -inf behind the row's end.  Rows begin at any address
@@ -139,11 +146,16 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p)
         bad = __syncthreads_or(bad);
         if (tid == 0) *out = ChunkStat{0.0, mx, bad ? -1 : min(min(s_a[0], s_a[1]), min(s_a[2], s_a[3]))};
     } else {
-        const double base = mx == -INFINITY ? 0.0 : (double)mx;
+        // (2^-1000 for what is smaller, -inf too: nothing beside the 1 of the maximum, and a chunk of -inf is not summed)
         double z = 0;
+        bool bad = mx == INFINITY;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) z += exp_neg(((double)x[k] - base) * p.inv_t);
-        z = wave_sum_d(z);
+        for (int k = 0; k < PER; k += 2) bad |= (bool)__builtin_isunordered(x[k], x[k + 1]);
+        if (mx != -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k) z += pow2_near(fmax((double)x[k] - (double)mx, p.least), p.per_t);
+        }
+        z = wave_sum_d(bad ? (double)NAN : z);
         if (lane == 0) s_z[wave] = z;
         __syncthreads();
         if (tid == 0) *out = ChunkStat{(s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), mx, 0};
@@ -151,17 +163,17 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p)
 }
 
 // maximum and sum of a whole row from its chunks, by 16 lanes, the same in all of them and -- the order being fixed -- in all workgroups
-__device__ __forceinline__ void join_row(const ChunkStat* st, int chunks, double inv_t, float& m, double& z)
+__device__ __forceinline__ void join_row(const VerifyParams& p, const ChunkStat* st, float& m, double& z)
 {
     const int lane = threadIdx.x & 15;
     m = -INFINITY;
-    for (int c = lane; c < chunks; c += 16) m = fmaxf(m, st[c].mx);
+    for (int c = lane; c < p.chunks; c += 16) m = fmaxf(m, st[c].mx);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     z = 0;
-    for (int c = lane; c < chunks; c += 16) {
+    for (int c = lane; c < p.chunks; c += 16) {
         const ChunkStat s = st[c];
-        z += s.mx == -INFINITY ? s.z : s.z * exp_neg(((double)s.mx - (double)m) * inv_t);    // (z of a chunk of -inf is 0, or NaN)
+        z += s.mx == -INFINITY ? s.z : s.z * pow2_neg((double)s.mx - (double)m, p);    // (z of a chunk of -inf is 0, or NaN)
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
@@ -170,7 +182,7 @@ __device__ __forceinline__ void join_row(const ChunkStat* st, int chunks, double
 // r: 1 / sum of the row's exponentials
 __device__ __forceinline__ double probability(const VerifyParams& p, float x, float m, double r)
 {
-    return p.probs ? (double)x : exp_neg(((double)x - (double)m) * p.inv_t) * r;
+    return p.probs ? (double)x : pow2_neg((double)x - (double)m, p) * r;
 }
 
 // How many of a sequence's tokens stand, and the rows that the next one is drawn from: by all 256 threads, the same in all of them.
@@ -194,8 +206,8 @@ template <typename T> __device__ __forceinline__ Chosen decide(const VerifyParam
             float m = 0;
             double z = 1;
             if (!p.probs) {
-                if (is_draft) join_row(p.d_stat + ((long)b * p.N + i) * p.chunks, p.chunks, p.inv_t, m, z);
-                else join_row(p.t_stat + ((long)b * (p.N + 1) + i) * p.chunks, p.chunks, p.inv_t, m, z);
+                if (is_draft) join_row(p, p.d_stat + ((long)b * p.N + i) * p.chunks, m, z);
+                else join_row(p, p.t_stat + ((long)b * (p.N + 1) + i) * p.chunks, m, z);
             }
             const double r = 1.0 / z;
             if ((tid & 15) == 0) {
@@ -301,7 +313,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
         if constexpr (!OWN) return mass[2 * c + which];
         if (which == 0 && ch.mode == 2 && c == point / CHUNK) return without;
         const ChunkStat s = st[c];
-        return (s.mx == -INFINITY ? s.z : s.z * exp_neg(((double)s.mx - (double)ch.mp) * p.inv_t)) * ch.rp;
+        return (s.mx == -INFINITY ? s.z : s.z * pow2_neg((double)s.mx - (double)ch.mp, p)) * ch.rp;
     };
     // totals: a thread a chunk, added up wave by wave in a fixed order
     double own[2] = {0, 0};
@@ -481,7 +493,8 @@ int uw_verify_draft(const uw_verify_args* a, void* stream)
     p.N = a->N;
     p.V = a->V;
     p.chunks = (int)chunks;
-    p.inv_t = greedy ? 0.0 : 1.0 / (double)a->temperature;
+    p.per_t = greedy ? 0.0 : 1.4426950408889634074 / (double)a->temperature;
+    p.least = greedy ? 0.0 : -1000.0 / p.per_t;
     p.probs = a->probs;
     p.accepted = a->accepted;
     p.tokens = a->tokens;
