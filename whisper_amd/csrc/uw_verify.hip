@@ -12,9 +12,10 @@
 // in L2 or the Infinity Cache by then); (3) a workgroup per sequence finds the chunk, then the token in it.  Probabilities need no
 // (1), logits without a draft no (2); greedy verification needs the arg-max of (1) and then one small launch.
 //
-// Measured: 64 windows, up to five tokens, both models' f32 logits (V 51865, 146 MB if all are read) 27 + 16 + 9.5 us: (1) 5.4 TB/s, (2) and
-// (3) chains of statistics, decision, scores and sums, for which few rows are left to work side by side.  One window of four tokens 4.1 + 12 us.
-// Greedy, 128 windows of four tokens, bf16 (66 MB) 17.6 + 4.0 us.
+// Measured: 64 windows of nought to five tokens, both models' f32 logits (V 51865, 80 MB read): 22.7 + 14.1 + 8.6 us.  (1) does as much f64
+// arithmetic as reading, 3.5 TB/s; (2) and (3) are chains of statistics, decision, scores and sums with few rows left to work side by side.
+// One window of four tokens 4.1 + 11.1 us.  Greedy, 128 windows of four tokens, bf16 (66 MB): 17.6 + 4.0 us, 3.8 TB/s.  Chunks of 2048 scores
+// take 26.4 + 14.2 + 7.7 us and greedy 24.2, of 8192 23.4 + 16.6 + 13.4 and 17.5.
 #include "../../include/uw_hip.h"
 #include "uw_common.h"
 #include "uw_kernels.h"
