@@ -137,3 +137,20 @@ def test_poisoned_blocks_and_missing_pages_reach_only_the_rows_that_see_them(dty
     assert not torch.isfinite(out[1, :, 0]).any() and torch.equal(out[1, :, 1:], clean[1, :, 1:])
     assert torch.isnan(out[2, at >= 320]).all() and torch.equal(out[2, at < 320], clean[2, at < 320])
     assert torch.isnan(out[3]).all()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_tables_far_wider_than_their_sequences(packed):
+    """One long sequence among many short ones, under a table that could hold half a million tokens: the scratch for its parts is
+    bounded, so its keys are cut more coarsely."""
+    g = _gen(51)
+    B, T, H, Hkv, D, P, kv = 128, 8, 4, 1, 64, 256, [90 + i % 50 for i in range(127)] + [20000]
+    c, table = _filled(g, B, 79, Hkv, D, P, "int8", kv)
+    wide = torch.full((B, 2000), -1, dtype=torch.int32, device=DEV)
+    wide[:, :79] = table
+    q = torch.randn(B, T, H, D, generator=g, device=DEV).to(BF)
+    start = [T * i for i in range(B + 1)] if packed else None
+    kw = {"tok_start": torch.tensor(start, dtype=torch.int32, device=DEV)} if packed else {}
+    x = q.flatten(0, 1) if packed else q
+    out, lse = kv8.attention(x, c, wide, torch.tensor(kv, dtype=torch.int32, device=DEV), return_lse=True, **kw)
+    _check(out, lse, x, c, wide, kv, "int8", True, D ** -0.5, start)

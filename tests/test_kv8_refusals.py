@@ -144,3 +144,17 @@ def test_verify_draft_refuses():
         assert lib.uw_verify_draft(_ARGS.pack(*{**good, **ws}.values()), None) > 0 and b"workspace" in lib.uw_last_error()
     assert lib.uw_verify_draft(_ARGS.pack(*{**good, "B": 1 << 20, "V": 51865}.values()), None) > 0 and b"too many rows" in lib.uw_last_error()
     assert lib.uw_verify_draft(None, None) > 0
+
+
+def test_attention_scratch_stays_small():
+    """Parts of cut sequences take at most 256 MB, whatever the table could hold."""
+    from whisper_amd import kv8
+    seen = set()
+    for B, T, heads, kv_heads, D, P, width in ((1, 1, 8, 1, 128, 64, 2000), (256, 4, 8, 1, 128, 256, 2000), (1, 2048, 8, 1, 128, 64, 8000),
+                                               (64, 1, 32, 8, 64, 16, 100000), (3, 200, 12, 12, 64, 64, 5000), (8, 5, 32, 8, 128, 64, 513)):
+        dims = kv8._CACHE_DIMS.pack(1000, kv_heads, P, D, 0, 0)
+        for packed in (False, True):
+            n = kv8._workspace_bytes(dims, B * T, width, B, 0 if packed else T, 1, packed, heads)
+            assert 0 <= n <= 256 << 20
+            seen.add(n > 0)
+    assert seen == {False, True}

@@ -768,7 +768,14 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
         // a tile's last item is a short one: they are counted in, so that all items find a place at once
         const long items = ceil_div(512, c->n_kv_heads);
         p.target = (int)std::max(std::max(items - p.groups, items / 2), 1l);
-        p.n_split = std::min(p.target, ceil_div(p.max_blocks, p.min_chunk));
+        // what one tile can be cut into: a chunk is at least the tiles' blocks over `target`
+        p.n_split = std::min(T > 0 ? ceil_div(p.target, p.tiles) : p.target, ceil_div(p.max_blocks, p.min_chunk));
+        // and what 256 MB of parts hold
+        const int hold = (int)std::max((int64_t)1, (int64_t)(256 << 20) / (n_tok * a->n_heads * (c->head_dim + 4) * 4));
+        if (hold < p.n_split) {
+            p.n_split = hold;
+            p.min_chunk = std::max(p.min_chunk, ceil_div(p.max_blocks, hold));
+        }
         if (p.n_split > 1) p.groups += p.target;
     }
     p.lds_rows = T > 0 ? (int)std::min((long)16 * p.rt, rows) : 16 * p.rt;
