@@ -199,3 +199,39 @@ def test_greedy_verification_of_an_engine():
     u = torch.rand(2, 6, generator=g, device=DEV)
     _check(logits, drafted, u, temperature=0.9)
     eng.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [8, 9, 17, 40])
+@pytest.mark.parametrize("mode", ["logits", "probs", "greedy"])
+def test_many_drafted_tokens(dtype, N, mode):
+    """A drafter that agrees up to a position of its own in every window: acceptance runs past eight positions, the last included."""
+    B, V = N + 1, 501
+    x, _, d, u = _inputs(70 + N, B, N, V, dtype, False)
+    d = x[:, :N].argmax(-1).to(torch.int32)
+    y = x[:, :N].clone()
+    for b in range(N):
+        y[b, b] = -1.0                                   # flat there,
+        x[b, b, d[b, b].long()] = -60.0                  # and the target has turned away from that token
+    t = 0.0 if mode == "greedy" else 1.0
+    if mode == "probs":
+        x, y = torch.softmax(x.float(), -1).to(dtype), torch.softmax(y.float(), -1).to(dtype)
+    acc, _ = _check(x, d, u, draft=y, temperature=t, probs=mode == "probs")
+    if mode != "greedy":
+        assert acc.tolist() == list(range(N + 1))
+    _check(x, d, u, temperature=t, probs=mode == "probs")
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-4, 0.05, 30.0, 1e6, 3e38])
+@pytest.mark.parametrize("with_draft", [False, True])
+def test_extreme_temperatures_and_masked_scores(temperature, with_draft):
+    """From arg-max to uniform over what is not masked; scores of -inf and of the type's lowest value are never drawn."""
+    B, N, V = 24, 3, 9001
+    x, y, d, u = _inputs(5, B, N, V, torch.float32, False)
+    for z in (x, y):
+        z[..., 1000:6000] = -float("inf")
+        z[..., 8000:] = torch.finfo(torch.float32).min if temperature < 1e5 else -float("inf")
+    d = torch.where((d >= 1000) & (d < 6000), d % 1000, d).to(torch.int32)
+    _, tok = _check(x, d, u, draft=y if with_draft else None, temperature=temperature)
+    got = tok[tok >= 0]
+    assert not ((got >= 1000) & (got < 6000)).any()
