@@ -46,7 +46,7 @@ struct AttnArgs {
     float* lse;
     const int32_t* kv_len;
     float* part;         // [rows][H][n_split][D + 4] partial results (output, its reference, sum, its reference) when n_split > 1
-    int H, G, causal;
+    int H, G, log2G, causal;   // log2G: -1 where G is no power of two
     int n_split;         // 1: an item is a row tile of a sequence; else at most so many items share a tile, each with a part of the keys
     int target, min_chunk;   // n_split > 1: items a head should come to, and the fewest blocks of 64 keys of one
     int tiles;           // row tiles per sequence (uniform)
@@ -170,6 +170,17 @@ __device__ __forceinline__ float across_groups_max(float x)
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
+// op over WK (4 or 8) neighbouring lanes' values, where those of a row of sixteen repeat after WK lanes
+template <int WK, typename OP> __device__ __forceinline__ float across_waves(float x, OP op)
+{
+#define KV8_ROTATED(n) x = op(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + n, 0xf, 0xf, true)))
+    if constexpr (WK == 8) KV8_ROTATED(4);
+    KV8_ROTATED(2);
+    KV8_ROTATED(1);
+#undef KV8_ROTATED
+    return x;
+}
+
 // what a wave, a workgroup or an item knows of a row beside its output
 struct RowState { float m, l, ms; };
 
@@ -187,7 +198,7 @@ __device__ __forceinline__ void result_of(const RowState& a, float& f0, float& f
 template <typename T, int D>
 __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first, int kvh, int row, int d, int split, int splits, RowState a, f32x4 acc)
 {
-    const int t = row / p.G, h = kvh * p.G + row % p.G;
+    const int t = p.log2G >= 0 ? row >> p.log2G : row / p.G, h = kvh * p.G + row - t * p.G;
     const long rg = t_first + t;                        // row of the call
     if (splits > 1) {
         float* at = p.part + ((rg * p.H + h) * p.n_split + split) * (D + 4);
@@ -271,40 +282,50 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 
     // keys each of this lane's rows sees; the fewest and the most of the wave's
     const int row_end = min(row0 + ROWS, n_rows);
-    auto seen = [&](int row) { return p.causal ? max(0, len - n + 1 + row / p.G) : len; };
+    auto token_of = [&](int row) { return p.log2G >= 0 ? row >> p.log2G : row / p.G; };
+    auto seen = [&](int row) { return p.causal ? max(0, len - n + 1 + token_of(row)) : len; };
     int lim[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) lim[i] = seen(min(row0 + 16 * i + rr, n_rows - 1));
     const int lim_min = row0 < n_rows ? seen(row0) : 0, lim_max = row0 < n_rows ? seen(row_end - 1) : 0;
 
-    // Q fragments
+    // the queries' bytes are asked for here and made into fragments once the first codes are on their way too
     bf16x8 qf[RT][HALF][2][NP];
+    uint4 q_raw[RT][HALF][2][sizeof(T) / 2];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int row = row0 + 16 * i + rr;
-        const int t = row / p.G, h = kvh * p.G + row % p.G;
-        const long at = (p.ts.tok_start ? (t_first + t) * p.q.sT : (long)b * p.q.sB + (long)t * p.q.sT) + (long)h * p.q.sH + g4 * 16;
+        const int row = row0 + 16 * i + rr, t = token_of(row), h = kvh * p.G + row - t * p.G;
+        const T* from = (const T*)p.q.data + (p.ts.tok_start ? (t_first + t) * p.q.sT : (long)b * p.q.sB + (long)t * p.q.sT) + (long)h * p.q.sH + g4 * 16;
 #pragma unroll
         for (int hf = 0; hf < HALF; ++hf)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if constexpr (NP == 1) {
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (row < n_rows) w = *(const uint4*)((const T*)p.q.data + at + hf * 64 + s * 8);
-                    const unsigned flip = p.neg | p.neg >> 16;
-                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-                    qf[i][hf][s][0] = __builtin_bit_cast(bf16x8, w);
-                } else {
-                    float x[8];
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = row < n_rows ? to_f32<T>(((const T*)p.q.data)[at + hf * 64 + s * 8 + e]) : 0.f;
-                        x[e] = __uint_as_float(__float_as_uint(x[e]) ^ p.neg);
-                    }
-                    planes<NP>(x, qf[i][hf][s]);
+                for (int u = 0; u < (int)sizeof(T) / 2; ++u) {
+                    q_raw[i][hf][s][u] = make_uint4(0, 0, 0, 0);
+                    if (row < n_rows) q_raw[i][hf][s][u] = *(const uint4*)(from + hf * 64 + s * 8 + u * 4);
                 }
-            }
     }
+    auto make_q = [&]() {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int hf = 0; hf < HALF; ++hf)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint4* w = q_raw[i][hf][s];
+                    if constexpr (NP == 1) {
+                        const unsigned flip = p.neg | p.neg >> 16;
+                        qf[i][hf][s][0] = __builtin_bit_cast(bf16x8, make_uint4(w[0].x ^ flip, w[0].y ^ flip, w[0].z ^ flip, w[0].w ^ flip));
+                    } else {
+                        const unsigned u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(u[e] ^ p.neg);
+                        planes<NP>(x, qf[i][hf][s]);
+                    }
+                }
+    };
 
     f32x4 o[RT][D / 16];
     float m[RT], l[RT], ms[RT];        // o holds weights * 2^-m, l weights * 2^-ms without the V scales (all in powers of two)
@@ -352,17 +373,20 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     const int v_row = (SHARE ? wr * 16 + rr : rr) * c.P, k_row = (SHARE ? 4 * wr + k_in : k_in) * D + g4 * 16;
 
     uint4 kf[4][HALF], vf[D / 16];
-    auto load_k = [&](int x) {
-        const int j = (x << 6) + k_group;
-        const uint8_t* kp = c.k + page_at(j) + ((j & (c.P - 1)) * D + k_row);
+    // where a lane's K and V of block x begin
+    auto find = [&](int x, const uint8_t*& kp, const uint8_t*& vp) {
+        const int jk = (x << 6) + k_group, jv = (x << 6) + 16 * g4;
+        const long pk = page_at(jk), pv = whole ? pk : page_at(jv);
+        kp = c.k + pk + ((jk & (c.P - 1)) * D + k_row);
+        vp = c.v + pv + ((jv & (c.P - 1)) + v_row);
+    };
+    auto load_k = [&](const uint8_t* kp) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int hf = 0; hf < HALF; ++hf) kf[t][hf] = ld_codes<(WR == 1)>(kp + t * 4 * D + hf * 64);
     };
-    auto load_v = [&](int x) {
-        const int j = (x << 6) + 16 * g4;
-        const uint8_t* vp = c.v + page_at(j) + ((j & (c.P - 1)) + v_row);
+    auto load_v = [&](const uint8_t* vp) {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(WR == 1)>(vp + d * 16 * c.P);
     };
@@ -375,9 +399,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     vtype* const v_ops = (vtype*)lds;
     uint4 raw[2 * HALF];
     auto bring = [&](int x) {
-        const int jk = (x << 6) + k_group, jv = (x << 6) + 16 * g4;
-        const long pk = page_at(jk), pv = whole ? pk : page_at(jv);
-        const uint8_t *kp = c.k + pk + ((jk & (c.P - 1)) * D + k_row), *vp = c.v + pv + ((jv & (c.P - 1)) + v_row);
+        const uint8_t *kp, *vp;
+        find(x, kp, vp);
 #pragma unroll
         for (int hf = 0; hf < HALF; ++hf) {
             raw[hf] = ld_codes<false>(kp + hf * 64);
@@ -401,16 +424,23 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     };
     if (!SHARE && blk < blk1) {
         window(blk);
-        load_k(blk);
-        load_v(blk);
+        const uint8_t *kp, *vp;
+        find(blk, kp, vp);
+        load_k(kp);
+        load_v(vp);
     }
+    make_q();
     // one step; MASK: some row does not see all 64 keys
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool mask = decltype(masked)::value;
         const int j0 = blk << 6, jv = j0 + 16 * g4;
         const bool more = !SHARE && blk + WK < blk1;
         const float kscale = __shfl(w_ks, at_key(jv), 64), lv = __shfl(w_lv, at_key(jv), 64);
-        if (more && !in_window(blk + WK)) window(blk + WK);
+        const uint8_t *k_next = nullptr, *v_next = nullptr;
+        if (more) {
+            if (!in_window(blk + WK)) window(blk + WK);
+            find(blk + WK, k_next, v_next);
+        }
         const int from = (blk & 1) * BUFFER + lane;      // SHARE
 
         f32x4 st[RT][4];
@@ -440,7 +470,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             }
         if constexpr (!SHARE) {
             __builtin_amdgcn_sched_barrier(0);
-            if (more) load_k(blk + WK);          // in flight under the softmax and P.V
+            if (more) load_k(k_next);          // in flight under the softmax and P.V
             __builtin_amdgcn_sched_barrier(0);
         }
 
@@ -543,7 +573,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         }
         if constexpr (!SHARE) {
             __builtin_amdgcn_sched_barrier(0);
-            if (more) load_v(blk + WK);
+            if (more) load_v(v_next);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -605,20 +635,31 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         __syncthreads();
         for (int e = (wk * 64 + lane) * 4; e < (row_end - row0) * D; e += 64 * WK * 4) {
             const int r = e / D, d = e % D;
-            RowState a = {-INFINITY, 0.f, -INFINITY};
+            // lane w of every eight (four) weighs wave w's part of the row: sixteen lanes or more have a row
+            const RowState x = sr[(lane & (WK - 1)) * R + r];
+            RowState a;
+            auto larger = [](float p, float q) { return fmaxf(p, q); };
+            a.m = across_waves<WK>(x.m, larger);
+            a.ms = across_waves<WK>(x.ms, larger);
+            // a wave without a finite score has a sum of 0, or NaN where it met a NaN
+            a.l = across_waves<WK>(x.l * (x.ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.ms - a.ms)), [](float p, float q) { return p + q; });
+            const float f = x.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.m - a.m);
             f32x4 acc = {0, 0, 0, 0};
-            for (int w = 0; w < WK; ++w) {
-                a.m = fmaxf(a.m, sr[w * R + r].m);
-                a.ms = fmaxf(a.ms, sr[w * R + r].ms);
-            }
-            for (int w = 0; w < WK; ++w) {
-                // a wave without a finite score has a sum of 0, or NaN where it met a NaN
-                const RowState x = sr[w * R + r];
-                a.l += x.l * (x.ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.ms - a.ms));
-                const float f = x.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.m - a.m);
-                const float* y = so + ((long)w * R + r) * D + d;
+            auto add = [&](auto w) {
+                const float fw = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(f), 0x150 + w.value, 0xf, 0xf, true));   // lane w of the sixteen
+                const float* y = so + ((long)w.value * R + r) * D + d;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] += y[k] * f;
+                for (int k = 0; k < 4; ++k) acc[k] = fmaf(y[k], fw, acc[k]);
+            };
+            add(std::integral_constant<int, 0>{});
+            add(std::integral_constant<int, 1>{});
+            add(std::integral_constant<int, 2>{});
+            add(std::integral_constant<int, 3>{});
+            if constexpr (WK == 8) {
+                add(std::integral_constant<int, 4>{});
+                add(std::integral_constant<int, 5>{});
+                add(std::integral_constant<int, 6>{});
+                add(std::integral_constant<int, 7>{});
             }
             if constexpr (STEP) {
                 float f0, f1, lse;
@@ -895,6 +936,7 @@ int uw_kv8_attention(const uw_kv8_attention_args* a, void* stream)
     x.part = (float*)a->ws;
     x.H = a->n_heads;
     x.G = a->n_heads / a->cache.n_kv_heads;
+    x.log2G = (x.G & (x.G - 1)) ? -1 : __builtin_ctz(x.G);
     x.causal = a->causal;
     x.n_split = pl.n_split;
     x.target = pl.target;
