@@ -17,6 +17,7 @@ _FORMATS = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 _FORMAT_OF = {torch.int8: L.UW_KV8_INT8, torch.float8_e4m3fn: L.UW_KV8_E4M3}
 _DTYPES = {torch.float32: L.UW_DTYPE_F32, torch.bfloat16: L.UW_DTYPE_BF16}
 
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 # the argument structures of the C ABI behind their uw_kv8_cache
 _CACHE = Struct("@4P6i")
 _CACHE_DIMS = Struct("@6i")
@@ -32,13 +33,14 @@ class KV8Cache:
     __slots__ = ("k", "v", "k_scale", "v_scale", "_c", "_dev", "_h", "_d")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        fmt = _FORMAT_OF.get(k.dtype)
-        if fmt is None or v.dtype != k.dtype or k.dim() != 4:
+        dtype = k.dtype
+        fmt = _FORMAT_OF.get(dtype)
+        if fmt is None or v.dtype is not dtype or k.dim() != 4:
             raise ValueError(f"codes must be int8 or float8_e4m3fn tensors of four dimensions, got {k.dtype} {tuple(k.shape)} and {v.dtype}")
         n, h, p, d = k.shape
         if v.shape != (n, h, d, p):
             raise ValueError(f"v must be [{n}, {h}, {d}, {p}] (transposed inside the page), got {tuple(v.shape)}")
-        if k_scale.shape != (n, h) or v_scale.shape != (n, h) or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        if k_scale.shape != (n, h) or v_scale.shape != (n, h) or k_scale.dtype is not _F32 or v_scale.dtype is not _F32:
             raise ValueError(f"scales must be float32 [{n}, {h}]")
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("cache tensors must be contiguous")
@@ -66,39 +68,43 @@ class KV8Cache:
     head_dim = property(lambda self: self.k.shape[3])
 
 
+# The checks come in an order that lets a sound argument through with the fewest questions: a call's arguments cost as much time as its
+# kernel when there is little to do.
 def _index(x: torch.Tensor, n: int, what: str, dev: int) -> torch.Tensor:
+    if x.dtype is _I32 and x.dim() == 1 and x.numel() == n and x.get_device() == dev and x.is_contiguous():
+        return x
     if x.shape != (n,) or x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what} must be an int32 tensor of {n} elements, got {x.dtype} {tuple(x.shape)}")
     if x.get_device() != dev:
         raise ValueError(f"{what} is on {x.device}, not on the cache's device")
-    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+    return x.to(torch.int32).contiguous()
 
 
-def _tokens(x: torch.Tensor, what: str, cache: KV8Cache, B: int, packed: bool):
-    """x [B, T, heads, head_dim], or [N, heads, head_dim] if packed -> the tensor to keep alive and (address, strides)."""
-    st = x.stride()
-    if len(st) != (3 if packed else 4) or x.dtype not in _DTYPES or x.shape[-1] != cache._d:
+def _tokens(x: torch.Tensor, shape: torch.Size, what: str, cache: KV8Cache, B: int, packed: bool):
+    """x [B, T, heads, head_dim], or [N, heads, head_dim] if packed -> the tensor to keep alive, its type and (address, strides)."""
+    st, dtype = x.stride(), x.dtype
+    code, unit = (L.UW_DTYPE_BF16, 7) if dtype is _BF16 else (L.UW_DTYPE_F32, 3) if dtype is _F32 else (-1, 0)
+    if len(st) != (3 if packed else 4) or code < 0 or shape[-1] != cache._d:
         raise ValueError(f"{what} must be float32 or bfloat16 " + ("[rows, heads, " if packed else "[B, T, heads, ")
-                         + f"{cache._d}], got {x.dtype} {tuple(x.shape)}")
-    if not packed and x.shape[0] != B:
-        raise ValueError(f"{what} holds {x.shape[0]} sequences, the page table {B}")
+                         + f"{cache._d}], got {dtype} {tuple(shape)}")
+    if not packed and shape[0] != B:
+        raise ValueError(f"{what} holds {shape[0]} sequences, the page table {B}")
     if x.get_device() != cache._dev:
         raise ValueError(f"{what} is on {x.device}, not on the cache's device")
     at = x.data_ptr()
-    unit = 7 if x.dtype is torch.bfloat16 else 3                # elements in 16 bytes, less one
-    if st[-1] != 1 or at & 15 or (st[-2] | st[-3] | st[0]) & unit:
+    if st[-1] != 1 or at & 15 or (st[-2] | st[-3] | st[0]) & unit:      # unit: elements in 16 bytes, less one
         x = x.clone(memory_format=torch.contiguous_format)      # rows the kernels cannot fetch in 16-byte pieces
         st, at = x.stride(), x.data_ptr()
-    return x, ((at, 0, st[0], st[1]) if packed else (at, st[0], st[1], st[2]))
+    return x, code, ((at, 0, st[0], st[1]) if packed else (at, st[0], st[1], st[2]))
 
 
 def _table(table: torch.Tensor, cache: KV8Cache) -> Tuple[int, int]:
-    shape = table.shape
-    if len(shape) != 2 or 0 in shape or table.dtype != torch.int32 or not table.is_contiguous():
-        raise ValueError(f"the page table must be a contiguous int32 tensor [B, blocks], got {table.dtype} {tuple(shape)}")
+    B, width = table.shape if table.dim() == 2 else (0, 0)
+    if not B or not width or table.dtype is not _I32 or not table.is_contiguous():
+        raise ValueError(f"the page table must be a contiguous int32 tensor [B, blocks], got {table.dtype} {tuple(table.shape)}")
     if table.get_device() != cache._dev:
         raise ValueError(f"the page table is on {table.device}, not on the cache's device")
-    return shape
+    return B, width
 
 
 # the current stream's handle: what torch.cuda.current_stream(dev).cuda_stream answers, without making a Stream object (2.7 us a call)
@@ -133,12 +139,12 @@ def append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, table: torch.Tenso
     shape = k.shape
     if shape != v.shape or k.dtype != v.dtype or len(shape) < 3 or shape[-2] != cache._h:
         raise ValueError(f"k and v must be alike, with {cache._h} heads: got {k.dtype} {tuple(shape)} and {v.dtype} {tuple(v.shape)}")
-    k, ck = _tokens(k, "k", cache, B, packed)
-    v, cv = _tokens(v, "v", cache, B, packed)
+    k, dtype, ck = _tokens(k, shape, "k", cache, B, packed)
+    v, _, cv = _tokens(v, shape, "v", cache, B, packed)
     _on_gpu(cache)
     n, T = (shape[0], 0) if packed else (B * shape[1], shape[1])
     _call(L.load().uw_kv8_append, cache._c + _STORE.pack(table.data_ptr(), pos.data_ptr(), tok_start.data_ptr() if packed else 0, n, width,
-                                                         B, T, _DTYPES[k.dtype], *ck, *cv), dev)
+                                                         B, T, dtype, *ck, *cv), dev)
 
 
 def read(cache: KV8Cache, table: torch.Tensor, first: torch.Tensor, n_tok: int, tok_start: Optional[torch.Tensor] = None,
@@ -156,7 +162,8 @@ def read(cache: KV8Cache, table: torch.Tensor, first: torch.Tensor, n_tok: int, 
         tok_start = _index(tok_start, B + 1, "tok_start", dev)
     _on_gpu(cache)
     h, d = cache._h, cache._d
-    k, v = cache.k_scale.new_empty((2, n_tok, h, d) if packed else (2, B, n_tok, h, d), dtype=dtype).unbind(0)
+    k = cache.k_scale.new_empty((n_tok, h, d) if packed else (B, n_tok, h, d), dtype=dtype)
+    v = torch.empty_like(k)
     st = (0, h * d, d) if packed else (n_tok * h * d, h * d, d)
     _call(L.load().uw_kv8_read, cache._c + _STORE.pack(table.data_ptr(), first.data_ptr(), tok_start.data_ptr() if packed else 0,
                                                        n_tok if packed else B * n_tok, width, B, 0 if packed else n_tok, _DTYPES[dtype],
@@ -187,19 +194,18 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
     packed = tok_start is not None
     if packed:
         tok_start = _index(tok_start, B + 1, "tok_start", dev)
-    q, cq = _tokens(q, "q", cache, B, packed)
     shape = q.shape
-    heads, d = shape[-2], shape[-1]
+    q, dtype, cq = _tokens(q, shape, "q", cache, B, packed)
+    heads, d = shape[-2], cache._d
     if heads % cache._h or heads == 0:
         raise ValueError(f"{heads} query heads over {cache._h} cached heads")
     if out is not None and (out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() & 15):
         raise ValueError("out must be contiguous, 16-byte aligned and like q")
     _on_gpu(cache)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = cache.k_scale.new_empty(shape[:-1]) if return_lse else None
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
     n, T = (shape[0], 0) if packed else (B * shape[1], shape[1])
-    dtype = _DTYPES[q.dtype]
+    lse = cache.k_scale.new_empty((n, heads) if packed else (B, T, heads)) if return_lse else None
     need = _workspace_bytes(cache._c[_ADDRESSES:], n, width, B, T, dtype, packed, heads)
     ws = cache.k_scale.new_empty(need // 4) if need else None
     _call(L.load().uw_kv8_attention, cache._c + _ATTEND.pack(
