@@ -100,12 +100,57 @@ template <typename T> __device__ __forceinline__ void load_scores(const T* row, 
     }
 }
 
-__device__ __forceinline__ double wave_sum_d(double v)
+// Sums and extremes over a wave or over sixteen lanes, by moves inside the vector ALU (a trip through LDS for each step would make up a
+// third of the small launches).  Their order is fixed, and the same for every lane that gets the result.
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double moved(double v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, true),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ double lane_d(double v, int lane)
+{
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+// sums of lanes 0 .. own: shifts inside the rows of sixteen, then the rows' totals handed on
+__device__ __forceinline__ double wave_sums_d(double v)
+{
+    v += moved<0x111>(v);
+    v += moved<0x112>(v);
+    v += moved<0x114>(v);
+    v += moved<0x118>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
     return v;
 }
+__device__ __forceinline__ double wave_sum_d(double v) { return lane_d(wave_sums_d(v), 63); }
+__device__ __forceinline__ double row_sum_d(double v)
+{
+    v += moved<0x128>(v);
+    v += moved<0x124>(v);
+    v += moved<0x122>(v);
+    v += moved<0x121>(v);
+    return v;
+}
+template <typename OP> __device__ __forceinline__ unsigned across_row(unsigned x, OP op)
+{
+    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+    return op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+}
+template <typename OP> __device__ __forceinline__ unsigned across_wave(unsigned x, OP op)
+{
+    x = across_row(x, op);
+    auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = op(a[0], a[1]);
+    a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return op(a[0], a[1]);
+}
+__device__ __forceinline__ unsigned larger_f(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+__device__ __forceinline__ float row_max_f(float x) { return __uint_as_float(across_row(__float_as_uint(x), larger_f)); }
+__device__ __forceinline__ float wave_max_f(float x) { return __uint_as_float(across_wave(__float_as_uint(x), larger_f)); }
+__device__ __forceinline__ int wave_min_i(int x) { return (int)across_wave((unsigned)x, [](unsigned a, unsigned b) { return (unsigned)min((int)a, (int)b); }); }
+__device__ __forceinline__ int wave_max_i(int x) { return (int)across_wave((unsigned)x, [](unsigned a, unsigned b) { return (unsigned)max((int)a, (int)b); }); }
 
 // (1) grid (chunks, B * (N + 1) target rows, then B * N draft rows)
 template <typename T, bool GREEDY>
@@ -128,7 +173,7 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p)
     float mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < PER; ++k) mx = fmaxf(mx, x[k]);
-    mx = wave_max(mx);
+    mx = wave_max_f(mx);
     if (lane == 0) s_m[wave] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
@@ -141,8 +186,7 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p)
             if (x[k] == mx) arg = score_index<T>(j0, k);            // a thread's indexes ascend with k
             bad |= x[k] != x[k];
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
+        arg = wave_min_i(arg);
         if (lane == 0) s_a[wave] = arg;
         bad = __syncthreads_or(bad);
         if (tid == 0) *out = ChunkStat{0.0, mx, bad ? -1 : min(min(s_a[0], s_a[1]), min(s_a[2], s_a[3]))};
@@ -169,15 +213,13 @@ __device__ __forceinline__ void join_row(const VerifyParams& p, const ChunkStat*
     const int lane = threadIdx.x & 15;
     m = -INFINITY;
     for (int c = lane; c < p.chunks; c += 16) m = fmaxf(m, st[c].mx);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    m = row_max_f(m);
     z = 0;
     for (int c = lane; c < p.chunks; c += 16) {
         const ChunkStat s = st[c];
         z += s.mx == -INFINITY ? s.z : s.z * pow2_neg((double)s.mx - (double)m, p);    // (z of a chunk of -inf is 0, or NaN)
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+    z = row_sum_d(z);
 }
 
 // r: 1 / sum of the row's exponentials
@@ -335,12 +377,19 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
         int at = -1, last = 0;
         for (int c0 = 0; c0 < p.chunks && at < 0; c0 += 64) {
             const double w = c0 + lane < p.chunks ? mass_of(c0 + lane, which) : 0.0;
-            for (int k = 0; k < min(64, p.chunks - c0); ++k) {
-                const double wk = __shfl(w, k, 64);
-                if (wk > 0) { last = c0 + k; last_before = cum; }
-                if (cum + wk > r) { at = c0 + k; before = cum; break; }
-                cum += wk;
+            const double incl = cum + wave_sums_d(w), excl = incl - w;
+            const unsigned long long some = __ballot(w > 0), over = __ballot(w > 0 && incl > r);
+            if (some) {
+                const int k = 63 - __clzll((long long)some);
+                last = c0 + k;
+                last_before = lane_d(excl, k);
             }
+            if (over) {
+                const int k = __ffsll((long long)over) - 1;
+                at = c0 + k;
+                before = lane_d(excl, k);
+            }
+            cum = lane_d(incl, 63);
         }
         if (lane == 0) {
             s_chunk = at < 0 ? last : at;
@@ -378,12 +427,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
         w[k] = v;
         sum += v;
     }
-    double incl = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += up;
-    }
+    double incl = wave_sums_d(sum);
     if (lane == 63) s_c[wave] = incl;
     __syncthreads();
     for (int k = 0; k < wave; ++k) incl += s_c[k];
@@ -395,11 +439,8 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyParams p)
         if (w[k] > 0) last = b0 + k;
         if (w[k] > 0 && cum > s_r) found = min(found, b0 + k);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        found = min(found, __shfl_xor(found, o, 64));
-        last = max(last, __shfl_xor(last, o, 64));
-    }
+    found = wave_min_i(found);
+    last = wave_max_i(last);
     if (lane == 0) { s_last[wave] = last; atomicMin(&s_next, found); }      // (a minimum: the order of arrival is nothing to it)
     __syncthreads();
     const int next = s_next != 0x7fffffff ? s_next : max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
@@ -424,10 +465,9 @@ __global__ __launch_bounds__(256) void verify_greedy_kernel(VerifyParams p)
                 bad |= s.arg < 0;
                 if (s.mx > m || arg == 0x7fffffff) { m = s.mx; arg = s.arg; }      // chunks ascend: the first of equal ones stays
             }
-            const float top = wave_max(m);
+            const float top = wave_max_f(m);
             if (m != top) arg = 0x7fffffff;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
+            arg = wave_min_i(arg);
             if (__any(bad)) arg = -1;
         }
         if (lane == 0) s_a[wave] = arg;
