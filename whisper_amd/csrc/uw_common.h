@@ -182,6 +182,22 @@ __device__ __forceinline__ float wave_max(float v)
     return v;
 }
 
+// op over the sixteen lanes of a row, and over the wave, by moves inside the vector ALU; every lane gets the result
+template <typename OP> __device__ __forceinline__ unsigned across_row(unsigned x, OP op)
+{
+    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+    return op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+}
+template <typename OP> __device__ __forceinline__ unsigned across_wave(unsigned x, OP op)
+{
+    x = across_row(x, op);
+    auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = op(a[0], a[1]);
+    a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return op(a[0], a[1]);
+}
 // First index of the maximum of row[0..V) (numpy argmax tie rule), computed by a 1024-thread workgroup: 16-byte loads,
 // eight independent loads in flight per thread.  sv / si: 16-entry LDS scratch.  The result is valid in thread 0 (after
 // the internal barrier); row must be 16-byte aligned for the vector path.  A NaN never wins the comparison; *any_nan

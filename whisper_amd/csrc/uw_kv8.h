@@ -179,8 +179,7 @@ template <typename CNT> __device__ __forceinline__ bool locate_from_end(int idx,
             most = max(most, n[i]);
         }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    most = (int)across_wave((unsigned)most, [](unsigned p, unsigned q) { return max(p, q); });
     // parts of the first r rounds
     auto dealt = [&](int r) { return __builtin_amdgcn_readlane(wave_scan((min(n[0], r) + min(n[1], r)) + (min(n[2], r) + min(n[3], r))), 63); };
     if (dealt(most) <= idx) return false;

@@ -130,8 +130,7 @@ __global__ __launch_bounds__(TPB) void kv8_append_kernel(Kv8View c, TokSpan ts, 
     const int h = blockIdx.x % c.Hkv, tid = threadIdx.x, P = c.P;
     const long src = k.row + (long)h * a.sH;
     auto block_max = [&](unsigned mx) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
+        mx = across_wave(mx, [](unsigned p, unsigned q) { return max(p, q); });
         if constexpr (TPB > 64) {
             if ((tid & 63) == 0) s_max[tid >> 6] = mx;
             __syncthreads();

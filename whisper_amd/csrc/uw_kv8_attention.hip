@@ -709,9 +709,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p, int tile_rows
         // the last sequence that begins at or before the row (those behind it are empty or later)
         int n = 0;
         for (int i = lane; i < p.ts.B; i += 64) n += p.ts.tok_start[i] <= row ? 1 : 0;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-        b = n - 1;
+        b = __builtin_amdgcn_readlane(wave_scan(n), 63) - 1;
         if (b < 0 || row >= p.ts.tok_start[b] + (long)p.ts.count(b)) return;
     } else {
         b = (int)(row / p.ts.T);
@@ -726,8 +724,9 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs p, int tile_rows
         a.m = fmaxf(a.m, part[s * (D + 4) + D]);
         a.ms = fmaxf(a.ms, part[s * (D + 4) + D + 2]);
     }
-    a.m = wave_max(a.m);
-    a.ms = wave_max(a.ms);
+    auto larger = [](unsigned x, unsigned y) { return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y))); };
+    a.m = __uint_as_float(across_wave(__float_as_uint(a.m), larger));
+    a.ms = __uint_as_float(across_wave(__float_as_uint(a.ms), larger));
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         const float* x = part + s * (D + 4);

@@ -131,21 +131,6 @@ __device__ __forceinline__ double row_sum_d(double v)
     v += moved<0x121>(v);
     return v;
 }
-template <typename OP> __device__ __forceinline__ unsigned across_row(unsigned x, OP op)
-{
-    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
-    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
-    x = op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
-    return op(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
-}
-template <typename OP> __device__ __forceinline__ unsigned across_wave(unsigned x, OP op)
-{
-    x = across_row(x, op);
-    auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = op(a[0], a[1]);
-    a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return op(a[0], a[1]);
-}
 __device__ __forceinline__ unsigned larger_f(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
 __device__ __forceinline__ float row_max_f(float x) { return __uint_as_float(across_row(__float_as_uint(x), larger_f)); }
 __device__ __forceinline__ float wave_max_f(float x) { return __uint_as_float(across_wave(__float_as_uint(x), larger_f)); }
