@@ -17,7 +17,7 @@ __device__ __forceinline__ int touched(int pos, int n, int log2P)
 // not each hold four waves).  Both are bound by memory: values once, codes once, nothing between.  V passes through LDS on its way to
 // or from [D][P], a channel's tokens at a pitch of P + 4 bytes, so that the words of a wave fall into different banks.
 // Measured: 32 x 1500 tokens of 12 heads of 64, bf16 (221 MB each way) stored in 53 us, 4.2 TB/s, read back in 44, 5.0 TB/s (a large copy:
-// 4.65); the newest token of 128 sequences stored in 8.2 us, which is one chain of length, page, value and scale, not bandwidth (0.6 MB).
+// 4.65); the newest token of 128 sequences stored in 7.8 us, which is one chain of length, page, value and scale, not bandwidth (0.6 MB).
 
 struct Block {           // one block of a call
     int b, r0, rows;            // sequence, first row in the block, rows of the call

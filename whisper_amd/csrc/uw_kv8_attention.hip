@@ -21,10 +21,11 @@ namespace {
 // three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a third of the bf16 rate.
 //
 // What bounds it: few rows of a head -- the stream of codes; 128 windows' token over 1500 keys of 12 heads (296 MB) 48.8 us, 6.1 TB/s; five
-// tokens of 4 heads a kv head over long ragged tables (297 MB) 58.6 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
+// tokens of 4 heads a kv head over long ragged tables (297 MB) 57.7 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
 // which has a multiply-add, an exponential (a quarter of the rate), an addition and half a conversion to do for each weight, beside the
 // 128 or 256 multiply-adds of the matrix unit: 33380 causal rows of 4 heads over 5000 keys 144 us, 750 TFLOP/s; of 128 channels 242 us,
-// 890.  One window -- a chain of lengths, pages, codes and the join of eight waves: 9.9 us.
+// 890.  One window of 6 heads -- a chain of lengths, pages, codes, three blocks a wave and the join of eight waves: 8.9 us (e4m3 7.4; int8's
+// conversions are the rest).  170 f32 rows of 64 heads over 1500 keys: 29 us, 140 TFLOP/s, three times that on the matrix unit.
 //
 // What a decoder step adds: one query token per window, its output in the operand layout of the product that follows, and the
 // probabilities of the alignment heads.

@@ -12,10 +12,10 @@
 // in L2 or the Infinity Cache by then); (3) a workgroup per sequence finds the chunk, then the token in it.  Probabilities need no
 // (1), logits without a draft no (2); greedy verification needs the arg-max of (1) and then one small launch.
 //
-// Measured: 64 windows of nought to five tokens, both models' f32 logits (V 51865, 80 MB read): 22.7 + 14.1 + 8.6 us.  (1) does as much f64
-// arithmetic as reading, 3.5 TB/s; (2) and (3) are chains of statistics, decision, scores and sums with few rows left to work side by side.
-// One window of four tokens 4.1 + 11.1 us.  Greedy, 128 windows of four tokens, bf16 (66 MB): 17.6 + 4.0 us, 3.8 TB/s.  Chunks of 2048 scores
-// take 26.4 + 14.2 + 7.7 us and greedy 24.2, of 8192 23.4 + 16.6 + 13.4 and 17.5.
+// Measured: 64 windows of nought to five tokens, both models' f32 logits (V 51865, 80 MB read): 21.1 + 13.4 + 7.6 us.  (1) does as much f64
+// arithmetic as reading, 3.8 TB/s; (2) and (3) are chains of statistics, decision, scores and sums with few rows left to work side by side.
+// One window of four tokens 3.7 + 8.8 us.  Greedy, 128 windows of four tokens, bf16 (66 MB): 15.9 + 3.9 us, 4.2 TB/s.  Chunks of 2048 scores
+// took 26.4 + 14.2 + 7.7 us and greedy 24.2, of 8192 23.4 + 16.6 + 13.4 and 17.5, when these took 22.7 + 14.1 + 8.6 and 17.8.
 #include "../../include/uw_hip.h"
 #include "uw_common.h"
 #include "uw_kernels.h"
@@ -47,7 +47,7 @@ struct VerifyParams {
 // 2^t, t = d * per_t, for -1000 <= t <= 0: 2^n 2^r with n the nearest whole number (what t + 1.5 2^52 has in its last bits), |r| <= 1/2;
 // 2^r by the polynomial that meets it at the nine Chebyshev nodes of [-1/2, 1/2], 1.1e-12 off at most; n added to the exponent.  That
 // moves one draw in ten million across a border between two tokens (2e-5 apart on average); the uniform numbers come in steps of 6e-8.
-// Twelve f64 instructions; they are what these kernels wait for as much as for memory (with eighteen, 64 windows took 48 us, now 43).
+// Twelve f64 instructions; they are what these kernels wait for as much as for memory (with eighteen, 64 windows took 48 us, with twelve 43).
 // A NaN stays one.
 __device__ __forceinline__ double pow2_near(double d, double per_t)
 {
