@@ -154,3 +154,47 @@ def test_tables_far_wider_than_their_sequences(packed):
     x = q.flatten(0, 1) if packed else q
     out, lse = kv8.attention(x, c, wide, torch.tensor(kv, dtype=torch.int32, device=DEV), return_lse=True, **kw)
     _check(out, lse, x, c, wide, kv, "int8", True, D ** -0.5, start)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kv,H,Hkv,D,T", [([100, 2500, 0, 64], 6, 2, 64, 1), ([100, 900], 15, 3, 64, 7), ([9000, 77], 7, 1, 128, 3),
+                                          ([300, 411, 257, 640], 48, 16, 64, 257), ([500, 130], 36, 12, 128, 600)])
+def test_query_heads_in_threes_fives_and_sevens(dtype, causal, kv, H, Hkv, D, T):
+    """Heads a kv head that are no power of two, in every shape of a call."""
+    g = _gen(H + D + T)
+    B, P = len(kv), 64
+    c, table = _filled(g, B, max(1, -(-max(kv) // P)), Hkv, D, P, "e4m3", kv)
+    q = torch.randn(B, T, H, D, generator=g, device=DEV).to(dtype)
+    out, lse = kv8.attention(q, c, table, torch.tensor(kv, dtype=torch.int32, device=DEV), causal=causal, return_lse=True)
+    _check(out, lse, q, c, table, kv, "e4m3", causal, D ** -0.5)
+
+
+def test_two_graphs_of_cut_sequences_with_lengths_that_change():
+    """Each graph has its own parts; lengths, tables and queries are read when it is replayed."""
+    g = _gen(61)
+    B, H, Hkv, D, P, T, longest = 3, 8, 2, 128, 64, 2, 9000
+    c, table = _filled(g, B, 141, Hkv, D, P, "int8", [longest] * B)
+    ln = torch.tensor([longest, 50, 4000], dtype=torch.int32, device=DEV)
+    qs = [torch.randn(B, T, H, D, generator=g, device=DEV).to(BF) for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kv8.attention(qs[0], c, table, ln)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, held = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(kv8.attention(q, c, table, ln, return_lse=True))
+    for kv in ([longest, 50, 4000], [0, 8999, 1], [70, 2112, 2113], [8192, 8192, 8192]):
+        ln.copy_(torch.tensor(kv, dtype=torch.int32))
+        for q in qs:
+            q.copy_(torch.randn(q.shape, generator=g, device=DEV))
+        for x in graphs:
+            x.replay()
+        for q, (out, lse) in zip(qs, held):
+            want, want_lse = kv8.attention(q, c, table, ln, return_lse=True)
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
+            torch.cuda.synchronize()
+            _check(out, lse, q, c, table, kv, "int8", True, D ** -0.5)
