@@ -217,7 +217,8 @@ typedef struct uw_kv8_attention_args {
 } uw_kv8_attention_args;
 
 /* Appends keys and values: sequence b's tokens go to positions len[b], len[b] + 1, ... (len = tokens already there).
- * Per touched block, head and half: a block without earlier tokens takes its scale from the largest |x|; otherwise the scale
+ * Per touched block, head and half: a block without earlier tokens takes its scale from the largest |x| (int8: |x| times the f32
+ * next to 1/127, 2^-126 at least; e4m3: the smallest power of two that leaves codes up to 448); otherwise the scale
  * stays while the new values fit and grows by a power of two if not, the earlier tokens' codes being re-rounded.  A NaN or
  * infinity makes the scale of its block and head NaN until the block is begun again: whatever reads that block gives NaN.
  * A block must not be touched by two sequences of one call (shared prefixes end on a page boundary).  Codes behind the last

@@ -22,7 +22,7 @@ def base_scale(amax, fmt):
     if amax == 0:
         return np.float32(0)
     if fmt == "int8":
-        return max(np.float32(np.float32(amax) / np.float32(127)), np.float32(2.0 ** -126))
+        return max(np.float32(amax) * np.float32(1 / 127), np.float32(2.0 ** -126))
     m, e = math.frexp(float(amax) / 448.0)
     return np.float32(2.0 ** max(e - 1 if m == 0.5 else e, -126))
 

@@ -4,7 +4,7 @@
 // transposed [D][P].  Both are then read along the index the attention product sums over -- D for q.k, the tokens for p.v -- as
 // 16-byte chunks that are MFMA operands as they lie, with no transpose between memory and register.  One f32 scale per page, head
 // and half; value = code * scale.  Two code formats, both exact in bf16 (8 significant bits):
-//   int8  codes -127 .. 127, scale = largest |x| / 127
+//   int8  codes -127 .. 127, scale = largest |x| times the f32 next to 1/127
 //   e4m3  (1-4-3, no infinities, largest 448), scale = the smallest power of two that fits
 #pragma once
 #include "../../include/uw_hip.h"
@@ -96,7 +96,7 @@ __device__ __forceinline__ int ceil_log2(double v)
 template <int F> __device__ __forceinline__ float kv8_base_scale(float amax)
 {
     if (!(amax > 0.f)) return 0.f;
-    if (F == UW_KV8_INT8) return fmaxf(amax / 127.0f, 0x1p-126f);
+    if (F == UW_KV8_INT8) return fmaxf(amax * (1.0f / 127.0f), 0x1p-126f);      // a product, as tensor libraries divide by a constant on GPUs
     return __uint_as_float((unsigned)(max(ceil_log2((double)amax / 448.0), -126) + 127) << 23);
 }
 // powers of two by which the scale s > 0 of a block with tokens in it has to grow for values up to amax (0: it fits).  Growing by
