@@ -16,16 +16,19 @@ namespace {
 // so neither K nor V nor P passes through LDS.  K scales multiply the scores, V scales ride in the exponent of the weights; one per 16
 // keys at least, so one per lane.  References, sums and outputs are f32.
 //
-// bf16 queries enter exactly.  Their weights are rounded once to f16 for P V -- 2^-11 of each at most, and 2^-25 of the largest where they run
-// out of exponent -- an eighth of what the bf16 result is rounded by; the codes are exact in f16 too.  f32 queries and weights enter as
-// three bf16 planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a third of the bf16 rate.
+// bf16 queries enter exactly, their weights as two bf16 planes: off by 2^-16 of each at most, with the whole of f32's exponent, so that
+// a row has its result to the same error when its largest weights meet values of zero.  (One f16 plane, which is faster -- 145 us for the
+// prompts below when this took 184, no difference where the stream of codes bounds -- loses the weights below 2^-25 of the largest and keeps
+// them in the sum.)  f32 queries and weights enter as three planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a
+// third of the bf16 rate.
 //
 // What bounds it: few rows of a head -- the stream of codes; 128 windows' token over 1500 keys of 12 heads (296 MB) 48.8 us, 6.1 TB/s; five
 // tokens of 4 heads a kv head over long ragged tables (297 MB) 57.7 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
-// which has a multiply-add, an exponential (a quarter of the rate), an addition and half a conversion to do for each weight, beside the
-// 128 or 256 multiply-adds of the matrix unit: 33380 causal rows of 4 heads over 5000 keys 144 us, 750 TFLOP/s; of 128 channels 242 us,
-// 890.  One window of 6 heads -- a chain of lengths, pages, codes, three blocks a wave and the join of eight waves: 8.9 us (e4m3 7.4; int8's
-// conversions are the rest).  170 f32 rows of 64 heads over 1500 keys: 29 us, 140 TFLOP/s, three times that on the matrix unit.
+// which has a multiply-add, an exponential (a quarter of the rate), an addition and the two planes to do for each weight, and the matrix
+// unit, with 192 or 384 multiply-adds for it: 33380 causal rows of 4 heads over 5000 keys 184 us, 590 TFLOP/s counted as 4 D
+// operations a weight.  One window of 6 heads -- a chain of lengths, pages, codes, three blocks a wave and the join of eight waves: 8.9 us
+// (e4m3 7.4; int8's conversions are the rest).  170 f32 rows of 64 heads over 1500 keys: 24.3 us, 170 TFLOP/s, three times that on the
+// matrix unit.
 //
 // What a decoder step adds: one query token per window, its output in the operand layout of the product that follows, and the
 // probabilities of the alignment heads.
@@ -83,46 +86,25 @@ template <> __device__ __forceinline__ bf16x8 codes8<UW_KV8_INT8>(unsigned a, un
     return v;
 }
 
-// the same in f16.  int8: 1024 + (code + 128) is f16 0x6400 | byte, so two bytes become two values by one byte permute and one packed
-// subtraction
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-template <int F> __device__ __forceinline__ f16x8 codes8h(unsigned a, unsigned b);
-template <> __device__ __forceinline__ f16x8 codes8h<UW_KV8_E4M3>(unsigned a, unsigned b)
-{
-    union { f16x2 p[4]; f16x8 v; } u;
-    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
-    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
-    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
-    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
-    return u.v;
-}
-template <> __device__ __forceinline__ f16x8 codes8h<UW_KV8_INT8>(unsigned a, unsigned b)
-{
-    union { f16x2 p[4]; f16x8 v; } u;
-    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
-    u.p[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400)) - off;
-    u.p[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402)) - off;
-    u.p[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400)) - off;
-    u.p[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402)) - off;
-    return u.v;
-}
-__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// the planes of 8 f32 values
-template <int NP> __device__ __forceinline__ void planes(const float* x, bf16x8* out)
+// The planes of 8 f32 values, each the rounded rest of those before.  DOT: the rest is taken from a packed pair by one dot product with
+// (-1, 0) or (0, -1), exact like the subtraction that needs the part unpacked first.
+template <int NP, bool DOT> __device__ __forceinline__ void planes(const float* x, bf16x8* out)
 {
+    unsigned own0 = 0x0000bf80u, own1 = 0xbf800000u;        // bf16 pairs (-1, 0), (0, -1)
+    asm("" : "+s"(own0), "+s"(own1));                       // in registers: as an inline constant the first is read as the second
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float rest = x[e];
+    for (int e = 0; e < 8; e += 2) {
+        float a = x[e], b = x[e + 1];
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            const __bf16 part = (__bf16)rest;
-            out[n][e] = part;
-            rest -= (float)part;
+            const bf16x2 part = {(__bf16)a, (__bf16)b};
+            out[n][e] = part[0];
+            out[n][e + 1] = part[1];
+            if (n + 1 == NP) continue;
+            a = DOT ? __builtin_amdgcn_fdot2_f32_bf16(part, __builtin_bit_cast(bf16x2, own0), a, false) : a - (float)part[0];
+            b = DOT ? __builtin_amdgcn_fdot2_f32_bf16(part, __builtin_bit_cast(bf16x2, own1), b, false) : b - (float)part[1];
         }
     }
 }
@@ -227,10 +209,11 @@ __device__ __forceinline__ void store_row(const AttnArgs& p, int b, long t_first
 template <int F, typename T, int D, int RT, int WK, int WR, bool STEP>
 __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 1 ? 4 : 3) : 2) void kv8_attention_kernel(AttnArgs p)
 {
-    constexpr int NP = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * RT, HALF = D / 64;
+    constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NW = sizeof(T) == 4 ? 3 : 2;       // planes of a query and of a weight
+    constexpr int ROWS = 16 * RT, HALF = D / 64;
+    constexpr bool DOT = WR == 4 || NQ == 3;
     constexpr bool SHARE = WR == 4;
     constexpr int BUFFER = 64 * D * 4 / 16;            // SHARE: 16-byte pieces of a block's operands
-    typedef typename std::conditional<NP == 1, f16x8, bf16x8>::type vtype;
     static_assert(WR == 1 || WK == 1, "waves share keys or stand side by side on rows");
     static_assert(WR == 1 || WR == 4, "");
     static_assert(!STEP || (D == 64 && RT == 1 && WK > 1), "a decoder step has one row of a head");
@@ -291,7 +274,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     const int lim_min = row0 < n_rows ? seen(row0) : 0, lim_max = row0 < n_rows ? seen(row_end - 1) : 0;
 
     // the queries' bytes are asked for here and made into fragments once the first codes are on their way too
-    bf16x8 qf[RT][HALF][2][NP];
+    bf16x8 qf[RT][HALF][2][NQ];
     uint4 q_raw[RT][HALF][2][sizeof(T) / 2];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -315,7 +298,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const uint4* w = q_raw[i][hf][s];
-                    if constexpr (NP == 1) {
+                    if constexpr (NQ == 1) {
                         const unsigned flip = p.neg | p.neg >> 16;
                         qf[i][hf][s][0] = __builtin_bit_cast(bf16x8, make_uint4(w[0].x ^ flip, w[0].y ^ flip, w[0].z ^ flip, w[0].w ^ flip));
                     } else {
@@ -323,7 +306,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
                         float x[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(u[e] ^ p.neg);
-                        planes<NP>(x, qf[i][hf][s]);
+                        planes<NQ, DOT>(x, qf[i][hf][s]);
                     }
                 }
     };
@@ -391,13 +374,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) vf[d] = ld_codes<(WR == 1)>(vp + d * 16 * c.P);
     };
-    auto v_operand = [&](unsigned x, unsigned y) {
-        if constexpr (NP == 1) return codes8h<F>(x, y);
-        else return codes8<F>(x, y);
-    };
     // SHARE: this wave's quarter of a block -- K tile wr, every fourth V tile from wr on
-    bf16x8* const k_ops = (bf16x8*)lds;                // [2 buffers][BUFFER / 2 of K, then as many of V]
-    vtype* const v_ops = (vtype*)lds;
+    bf16x8* const ops = (bf16x8*)lds;                  // [2 buffers][BUFFER / 2 of K, then as many of V]
     uint4 raw[2 * HALF];
     auto bring = [&](int x) {
         const uint8_t *kp, *vp;
@@ -417,10 +395,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         }
 #pragma unroll
         for (int hf = 0; hf < HALF; ++hf) {
-            k_ops[to + ((wr * HALF + hf) * 2) * 64] = codes8<F>(raw[hf].x, raw[hf].y);
-            k_ops[to + ((wr * HALF + hf) * 2 + 1) * 64] = codes8<F>(raw[hf].z, raw[hf].w);
-            v_ops[to + BUFFER / 2 + ((hf * 4 + wr) * 2) * 64] = v_operand(raw[HALF + hf].x, raw[HALF + hf].y);
-            v_ops[to + BUFFER / 2 + ((hf * 4 + wr) * 2 + 1) * 64] = v_operand(raw[HALF + hf].z, raw[HALF + hf].w);
+            ops[to + ((wr * HALF + hf) * 2) * 64] = codes8<F>(raw[hf].x, raw[hf].y);
+            ops[to + ((wr * HALF + hf) * 2 + 1) * 64] = codes8<F>(raw[hf].z, raw[hf].w);
+            ops[to + BUFFER / 2 + ((hf * 4 + wr) * 2) * 64] = codes8<F>(raw[HALF + hf].x, raw[HALF + hf].y);
+            ops[to + BUFFER / 2 + ((hf * 4 + wr) * 2 + 1) * 64] = codes8<F>(raw[HALF + hf].z, raw[HALF + hf].w);
         }
     };
     if (!SHARE && blk < blk1) {
@@ -455,8 +433,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             for (int hf = 0; hf < HALF; ++hf) {
                 bf16x8 a0, a1;
                 if constexpr (SHARE) {
-                    a0 = k_ops[from + ((t * HALF + hf) * 2) * 64];
-                    a1 = k_ops[from + ((t * HALF + hf) * 2 + 1) * 64];
+                    a0 = ops[from + ((t * HALF + hf) * 2) * 64];
+                    a1 = ops[from + ((t * HALF + hf) * 2 + 1) * 64];
                 } else {
                     a0 = codes8<F>(kf[t][hf].x, kf[t][hf].y);
                     a1 = codes8<F>(kf[t][hf].z, kf[t][hf].w);
@@ -464,7 +442,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
-                    for (int pl = NP - 1; pl >= 0; --pl) {
+                    for (int pl = NQ - 1; pl >= 0; --pl) {
                         st[i][t] = mfma(a0, qf[i][hf][0][pl], st[i][t]);
                         st[i][t] = mfma(a1, qf[i][hf][1][pl], st[i][t]);
                     }
@@ -475,7 +453,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        vtype pf[RT][2][NP];
+        bf16x8 pf[RT][2][NW];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int left = lim[i] - jv;          // keys of this lane's 16 that the row sees
@@ -535,19 +513,13 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             }
             // (a poisoned scale of a block that is seen shows in the sum)
             if (!mask || left > 0) l[i] = fmaf(sum, unit, l[i]);
-            // (f16 has nothing below 2^-25: weights of a V scale that was raised, at most 2^(30 - 64), are 0 there in any case)
-            if (NP > 1 && lw > lv) {
+            if (lw > lv) {
                 const float down = __builtin_amdgcn_exp2f(lv - lw);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) x[k] *= down;
             }
-            if constexpr (NP == 1) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) pf[i][k >> 3][0][k & 7] = (_Float16)x[k];
-            } else {
-                planes<NP>(x, pf[i][0]);
-                planes<NP>(x + 8, pf[i][1]);
-            }
+            planes<NW, DOT>(x, pf[i][0]);
+            planes<NW, DOT>(x + 8, pf[i][1]);
         }
         if constexpr (mask && !SHARE) {      // leftovers behind the sequence's end may hold NaN, which a weight of 0 does not silence
             const int keep = max(0, min(16, len - jv));
@@ -556,18 +528,18 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         }
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            vtype a0, a1;
+            bf16x8 a0, a1;
             if constexpr (SHARE) {
-                a0 = v_ops[from + BUFFER / 2 + (d * 2) * 64];
-                a1 = v_ops[from + BUFFER / 2 + (d * 2 + 1) * 64];
+                a0 = ops[from + BUFFER / 2 + (d * 2) * 64];
+                a1 = ops[from + BUFFER / 2 + (d * 2 + 1) * 64];
             } else {
-                a0 = v_operand(vf[d].x, vf[d].y);
-                a1 = v_operand(vf[d].z, vf[d].w);
+                a0 = codes8<F>(vf[d].x, vf[d].y);
+                a1 = codes8<F>(vf[d].z, vf[d].w);
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int pl = NP - 1; pl >= 0; --pl) {
+                for (int pl = NW - 1; pl >= 0; --pl) {
                     o[i][d] = mfma(a0, pf[i][0][pl], o[i][d]);
                     o[i][d] = mfma(a1, pf[i][1][pl], o[i][d]);
                 }
