@@ -328,8 +328,9 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     int blk = blk0 + wk;
 
     // 64 pages from the one of block `blk` on, one to a lane: where its codes begin, its K scale and the logarithm of its V scale, so that a
-    // step asks memory for nothing but codes and multiplies no addresses.  A page that does not exist is read as page 0 with NaN scales;
-    // a block of zeros (scale 0) has codes of zero, any scale does.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
+    // step asks memory for nothing but codes and multiplies no addresses.  A page that does not exist is read as page 0 with NaN scales.
+    // A block of zeros (scale 0) has codes of zero, any scale does for the product; the smallest there is keeps it from raising the reference m
+    // over the blocks that make the result.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
     int win = 0, w_lo = 0, w_hi = 0;
     float w_ks = 0.f, w_lv = 0.f;
     auto window = [&](int from) {
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         if (id >= 0) {
             const float vs = c.vs[at];
             w_ks = c.ks[at] * p.scale2;
-            w_lv = __builtin_amdgcn_logf(vs == 0.f ? 1.f : vs);
+            w_lv = __builtin_amdgcn_logf(vs == 0.f ? 0x1p-126f : vs);
         }
     };
     // whether the pages of block x are in it
