@@ -240,7 +240,8 @@ int uw_kv8_attention(const uw_kv8_attention_args* args, void* stream);
  * drafted i32 [B][N], n_drafted i32 [B] (NULL: N for all; clamped to 0..N), uniforms f32 [B][N+1] in [0, 1).
  * With p_i, q_i = softmax(row / temperature): token i is accepted while uniforms[b][i] * q_i(d_i) < p_i(d_i).  At the first
  * rejection the next token is drawn from max(p_i - q_i, 0), after the last accepted one from p_n: the smallest index whose
- * cumulative weight exceeds uniforms[b][N] times the whole.  All of this in 64 bits.  temperature 0: a token is accepted while it
+ * cumulative weight exceeds uniforms[b][N] times the whole.  All of this in 64-bit numbers, the temperature too; an exponential is off by
+ * 1.1e-12 at most.  temperature 0: a token is accepted while it
  * is its row's arg-max (the lowest index of equal ones) and the next token is the arg-max; draft and uniforms are not read.
  * accepted i32 [B]; tokens i32 [B][N+1]: the accepted tokens, the next token, then -1.  The next token is -1 if its row holds
  * a NaN or has no mass (the decoder-run failure of core.py:948-956); a drafted id outside 0..V-1 is never accepted.
@@ -257,8 +258,8 @@ typedef struct uw_verify_args {
     void* ws;
     int64_t ws_bytes;
     int32_t dtype, B, N, V;
-    float temperature;
-    int32_t probs;
+    double temperature;
+    int32_t probs, reserved;
 } uw_verify_args;
 int64_t uw_verify_draft_workspace_bytes(const uw_verify_args* args);
 int uw_verify_draft(const uw_verify_args* args, void* stream);

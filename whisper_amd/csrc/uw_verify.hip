@@ -470,10 +470,10 @@ __global__ __launch_bounds__(256) void verify_greedy_kernel(VerifyParams p)
 }
 
 long chunks_of(const uw_verify_args* a) { return ceil_div(a->V, CHUNK); }
-bool all_rows(const uw_verify_args* a) { return !a->probs || a->temperature == 0.f; }
+bool all_rows(const uw_verify_args* a) { return !a->probs || a->temperature == 0.0; }
 int64_t workspace_bytes(const uw_verify_args* a)
 {
-    const int64_t rows = all_rows(a) ? (int64_t)a->B * (a->N + 1 + (a->temperature > 0.f && a->draft ? a->N : 0)) : 0;
+    const int64_t rows = all_rows(a) ? (int64_t)a->B * (a->N + 1 + (a->temperature > 0.0 && a->draft ? a->N : 0)) : 0;
     return rows * chunks_of(a) * (int64_t)sizeof(ChunkStat) + (int64_t)a->B * (chunks_of(a) * 16 + (int64_t)sizeof(Chosen));
 }
 
@@ -484,9 +484,9 @@ int check_verify(const uw_verify_args* a)
     UW_REQUIRE(a->B > 0 && a->N >= 0 && a->V > 0, "uw_verify_draft: B %d, N %d, V %d", a->B, a->N, a->V);
     UW_REQUIRE(a->V <= 0x7fffffff - CHUNK && (double)a->B * (2.0 * a->N + 1) * ((a->V + CHUNK - 1) / CHUNK) < (1 << 24), "uw_verify_draft: too many rows");
     UW_REQUIRE(a->target && a->accepted && a->tokens && (a->drafted || a->N == 0), "uw_verify_draft: null argument");
-    UW_REQUIRE(a->temperature >= 0.f && a->temperature < INFINITY, "uw_verify_draft: temperature must be finite and not negative");
-    UW_REQUIRE(a->uniforms || a->temperature == 0.f, "uw_verify_draft: uniforms missing");
-    UW_REQUIRE(!a->probs || a->temperature == 1.f || a->temperature == 0.f, "uw_verify_draft: probabilities take no temperature");
+    UW_REQUIRE(a->temperature >= 0.0 && a->temperature < INFINITY, "uw_verify_draft: temperature must be finite and not negative");
+    UW_REQUIRE(a->uniforms || a->temperature == 0.0, "uw_verify_draft: uniforms missing");
+    UW_REQUIRE(!a->probs || a->temperature == 1.0 || a->temperature == 0.0, "uw_verify_draft: probabilities take no temperature");
     UW_REQUIRE((((uintptr_t)a->target | (uintptr_t)a->draft) & (a->dtype == UW_DTYPE_F32 ? 3 : 1)) == 0, "uw_verify_draft: misaligned rows");
     return UW_OK;
 }
@@ -503,7 +503,7 @@ int uw_verify_draft(const uw_verify_args* a, void* stream)
     if (rc) return rc;
     UW_REQUIRE(a->ws && ((uintptr_t)a->ws & 15) == 0 && a->ws_bytes >= workspace_bytes(a),
                "uw_verify_draft: workspace missing, misaligned or smaller than %lld bytes", (long long)workspace_bytes(a));
-    const bool greedy = a->temperature == 0.f;
+    const bool greedy = a->temperature == 0.0;
     const long chunks = chunks_of(a), t_rows = (long)a->B * (a->N + 1), d_rows = !greedy && a->draft ? (long)a->B * a->N : 0;
     VerifyParams p;
     p.target = a->target;
@@ -519,7 +519,8 @@ int uw_verify_draft(const uw_verify_args* a, void* stream)
     p.N = a->N;
     p.V = a->V;
     p.chunks = (int)chunks;
-    p.per_t = greedy ? 0.0 : 1.4426950408889634074 / (double)a->temperature;
+    // (beyond these bounds nothing changes: from 1e-60 down any two f32 scores that differ are 2^-1000 apart, from 1e60 up none are)
+    p.per_t = greedy ? 0.0 : 1.4426950408889634074 / std::min(std::max(a->temperature, 1e-60), 1e60);
     p.least = greedy ? 0.0 : -1000.0 / p.per_t;
     p.probs = a->probs;
     p.accepted = a->accepted;

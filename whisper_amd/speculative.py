@@ -13,7 +13,7 @@ from . import lib as L
 from .kv8 import _call
 
 _DTYPES = {torch.float32: L.UW_DTYPE_F32, torch.bfloat16: L.UW_DTYPE_BF16}
-_ARGS = Struct("@P2q P2q 5P Pq 4ifi")          # uw_verify_args
+_ARGS = Struct("@P2q P2q 5P Pq 4idi4x")        # uw_verify_args
 
 
 def _ints(x: torch.Tensor, shape, what: str, dev: int) -> torch.Tensor:
