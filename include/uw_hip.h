@@ -175,6 +175,8 @@ int uw_profile_span(uw_ctx* ctx, int kind, int64_t* launches_total, int64_t* lau
  *   k_scale, v_scale  f32 [n_pages][n_kv_heads];   value = code * scale
  * Formats: UW_KV8_INT8 (codes -127..127) and UW_KV8_E4M3 (1-4-3 without infinities, scales are powers of two).  page: 16, 32,
  * 64, 128 or 256; head_dim: 64 or 128.  k and v must be 16-byte aligned.
+ * (What a cache that was filled otherwise has to keep: codes of tokens are numbers, scales 0 -- all codes of the block 0 -- or 2^-126 at
+ * least, or NaN.  Codes behind a sequence's end may be anything.)
  * table i32 [B][table_width]: the page of each block of a sequence, block i holding positions i * page ... Entries behind a
  * sequence's end are not read.  A page id outside 0..n_pages-1, or a position before 0 or behind the table, is never accessed:
  * an append skips it, a read and an attention row that sees it give NaN.

@@ -246,6 +246,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         b = item % p.ts.B;
         tile = p.tiles - 1 - item / p.ts.B;
     }
+    // (the same in all lanes; in scalar registers what is kept over the loop spills nothing.  Not the first row of the side-by-side shape, nor the
+    // chunk: the loop is then compiled with a hundred registers spilled)
+    split = __builtin_amdgcn_readfirstlane(split);
+    splits = __builtin_amdgcn_readfirstlane(splits);
     if (STEP && p.step.active && !p.step.active[b]) return;
     // STEP: an alignment head's scores are kept in LDS (behind what the waves join there) until their sum is known
     float *scores = nullptr, *row_out = nullptr;
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         }
     }
     const int n = p.ts.count(b), n_rows = n * p.G;
-    const int row0 = (tile * WR + wr) * ROWS;
+    const int row0 = SHARE ? (tile * WR + wr) * ROWS : __builtin_amdgcn_readfirstlane((tile * WR + wr) * ROWS);
     const int len = max(0, p.kv_len[b]);
     const long t_first = p.ts.first(b);
 
@@ -324,18 +328,25 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     // blocks of 64 keys of this item, dealt to the waves
     const int blocks = min((lim_max >> 6) + ((lim_max & 63) ? 1 : 0), p.max_blocks);
     const int blk0 = split * chunk, blk1 = splits > 1 ? min(blocks, blk0 + chunk) : blocks;
+    // as far as the wave that sees most
+    const int tile_end = min((tile + 1) * WR * ROWS, n_rows), most = tile_end > 0 ? seen(tile_end - 1) : 0;
+    const int last = __builtin_amdgcn_readfirstlane(SHARE ? most : min(lim_max, blk1 << 6));      // keys from here on are nobody's
     const int k_group = 16 * (rr >> 2), k_in = rr & 3;     // 16-key group and place in it of this lane's K rows
     int blk = blk0 + wk;
 
     // 64 pages from the one of block `blk` on, one to a lane: where its codes begin, its K scale and the logarithm of its V scale, so that a
-    // step asks memory for nothing but codes and multiplies no addresses.  A page that does not exist is read as page 0 with NaN scales.
+    // step asks memory for nothing but codes and multiplies no addresses.  Entries behind the last key are not looked up.  In the place of a
+    // page that does not exist page 0 is read, with NaN scales and its V codes taken as 0: whatever they are, rows that see none of its keys
+    // keep their result.
     // A block of zeros (scale 0) has codes of zero, any scale does for the product; the smallest there is keeps it from raising the reference m
     // over the blocks that make the result.  (The rounding of log2(vs) adds |log2 vs| 2^-24 to a weight.)
     int win = 0, w_lo = 0, w_hi = 0;
     float w_ks = 0.f, w_lv = 0.f;
+    int clean = 0;           // up to here the window's V scales are numbers
     auto window = [&](int from) {
         win = (from << 6) >> c.log2P;
-        const int id = kv8_page(c, b, (long)win + lane);
+        const bool wanted = win + lane <= (last - 1) >> c.log2P;
+        const int id = wanted ? kv8_page(c, b, (long)win + lane) : -1;
         const long at = (long)max(id, 0) * c.Hkv + kvh, off = at * c.P * D;
         w_lo = (int)off;
         w_hi = (int)(off >> 32);
@@ -345,6 +356,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             w_ks = c.ks[at] * p.scale2;
             w_lv = __builtin_amdgcn_logf(vs == 0.f ? 0x1p-126f : vs);
         }
+        const unsigned long long odd = __ballot(wanted && w_lv != w_lv);
+        clean = odd ? min(last, (win + __ffsll((long long)odd) - 1) << c.log2P) : last;
     };
     // whether the pages of block x are in it
     auto in_window = [&](int x) { return (((x << 6) + 48) >> c.log2P) - win < 64; };
@@ -389,8 +402,10 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     };
     auto convert = [&](int x) {
         const int to = (x & 1) * BUFFER + lane;
-        if (len - (x << 6) < 64) {      // leftovers behind the sequence's end may hold NaN, which a weight of 0 does not silence
-            const int keep = max(0, min(16, len - ((x << 6) + 16 * g4)));
+        if (clean - (x << 6) < 64) {      // leftovers may hold NaN, which a weight of 0 does not silence
+            const int j = (x << 6) + 16 * g4;
+            const float lv = __shfl(w_lv, at_key(j), 64);
+            const int keep = lv != lv ? 0 : max(0, min(16, last - j));
 #pragma unroll
             for (int hf = 0; hf < HALF; ++hf) raw[HALF + hf] = first_bytes(raw[HALF + hf], keep);
         }
@@ -410,7 +425,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
         load_v(vp);
     }
     make_q();
-    // one step; MASK: some row does not see all 64 keys
+    // one step; MASK: some row does not see all 64 keys, or some of them have no page
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool mask = decltype(masked)::value;
         const int j0 = blk << 6, jv = j0 + 16 * g4;
@@ -522,8 +537,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
             planes<NW, DOT>(x, pf[i][0]);
             planes<NW, DOT>(x + 8, pf[i][1]);
         }
-        if constexpr (mask && !SHARE) {      // leftovers behind the sequence's end may hold NaN, which a weight of 0 does not silence
-            const int keep = max(0, min(16, len - jv));
+        if constexpr (mask && !SHARE) {      // leftovers may hold NaN, which a weight of 0 does not silence
+            const int keep = lv != lv ? 0 : max(0, min(16, last - jv));
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) vf[d] = first_bytes(vf[d], keep);
         }
@@ -553,16 +568,14 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
     };
     auto steps = [&](int end) {
         for (; blk < end; blk += WK) {
-            if (lim_min - (blk << 6) < 64) step(std::true_type{});
+            if ((SHARE ? lim_min : min(lim_min, clean)) - (blk << 6) < 64) step(std::true_type{});
             else step(std::false_type{});
         }
     };
     if constexpr (!SHARE) {
         steps(blk1);
     } else {
-        // as far as the wave that sees most
-        const int all_end = min((tile + 1) * WR * ROWS, n_rows);
-        const int most = all_end > 0 ? seen(all_end - 1) : 0, end = min((most >> 6) + ((most & 63) ? 1 : 0), p.max_blocks);
+        const int end = min((most >> 6) + ((most & 63) ? 1 : 0), p.max_blocks);
         if (end > 0) {
             window(0);
             bring(0);
