@@ -110,6 +110,7 @@ struct uw_ctx {
     int fused_logits = 1;          // up to 16 windows (bf16): LayerNorm + tied projection + arg-max candidates in one launch
     // 8-bit copy of the cross K/V that decode steps read (uw_ctx_cross_cache); pages of 64 frames, window b's at b * cross8_width ...
     int cross8_format = -1;        // -1: none, steps read cross_kv
+    uint8_t* cross8_block = nullptr;   // holds all of the following
     uint8_t* cross8_codes = nullptr;   // [Ld][K | V][Bm * cross8_width][H][64 * 64]
     float* cross8_scales = nullptr;    // [Ld][K | V][Bm * cross8_width][H]
     int32_t *cross8_table = nullptr, *cross8_len = nullptr, *cross8_pos = nullptr;   // [Bm][cross8_width]; [Bm] frames; [Bm] zeros
@@ -1032,15 +1033,18 @@ int uw_ctx_cross_cache(uw_ctx* c, int format)
     if (format >= 0 && !c->cross8_codes) {
         const int W = (c->S + 63) / 64;
         const size_t pages = (size_t)c->Bm * W, Ld = c->dec.size();
-        ALLOC(c->cross8_scales, Ld * 2 * pages * c->H * 4, true);
-        ALLOC(c->cross8_table, pages * 4, false);
-        ALLOC(c->cross8_len, (size_t)c->Bm * 4, false);
-        ALLOC(c->cross8_pos, (size_t)c->Bm * 4, true);
+        // one allocation, so that one that fails leaves nothing behind
+        const size_t codes = Ld * 2 * pages * c->H * 64 * 64, scales = Ld * 2 * pages * c->H * 4;
+        if (!c->cross8_block) ALLOC(c->cross8_block, codes + scales + (pages + 2 * (size_t)c->Bm) * 4, true);
+        c->cross8_scales = (float*)(c->cross8_block + codes);
+        c->cross8_table = (int32_t*)(c->cross8_block + codes + scales);
+        c->cross8_len = c->cross8_table + pages;
+        c->cross8_pos = c->cross8_len + c->Bm;
         hipLaunchKernelGGL(cross8_tables_kernel, dim3(ceil_div(pages, 256)), dim3(256), 0, nullptr, c->cross8_table, (int)pages, c->cross8_len, c->Bm, c->S);
         UW_LAUNCH_CHECK();
-        c->cross8_width = W;
-        ALLOC(c->cross8_codes, Ld * 2 * pages * c->H * 64 * 64, true);
         UW_HIP_CHECK(hipDeviceSynchronize());
+        c->cross8_width = W;
+        c->cross8_codes = c->cross8_block;
     }
     if (format != c->cross8_format) c->cross_batch = 0;      // the next uw_cross_kv fills it
     c->cross8_format = format;

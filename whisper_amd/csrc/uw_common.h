@@ -19,6 +19,7 @@ void uw_set_error(const char* fmt, ...);
         hipError_t e__ = (expr);                                                                      \
         if (e__ != hipSuccess) {                                                                      \
             uw_set_error("%s failed: %s (%s:%d)", #expr, hipGetErrorString(e__), __FILE__, __LINE__); \
+            (void)hipGetLastError(); /* told: not left for the next launch to find */                 \
             return UW_ERR_HIP;                                                                        \
         }                                                                                             \
     } while (0)
