@@ -70,6 +70,11 @@ class KV8Cache:
 
 # The checks come in an order that lets a sound argument through with the fewest questions: a call's arguments cost as much time as its
 # kernel when there is little to do.
+def narrowed(x: torch.Tensor) -> torch.Tensor:
+    """Whole numbers as contiguous int32; of 64 bits, those that 32 do not hold become the outermost that they do."""
+    return (x.clamp(-(1 << 31), (1 << 31) - 1) if x.dtype is torch.int64 else x).to(_I32).contiguous()
+
+
 def _index(x: torch.Tensor, n: int, what: str, dev: int) -> torch.Tensor:
     if x.dtype is _I32 and x.dim() == 1 and x.numel() == n and x.get_device() == dev and x.is_contiguous():
         return x
@@ -77,7 +82,7 @@ def _index(x: torch.Tensor, n: int, what: str, dev: int) -> torch.Tensor:
         raise ValueError(f"{what} must be an int32 tensor of {n} elements, got {x.dtype} {tuple(x.shape)}")
     if x.get_device() != dev:
         raise ValueError(f"{what} is on {x.device}, not on the cache's device")
-    return x.to(torch.int32).contiguous()
+    return narrowed(x)
 
 
 def _tokens(x: torch.Tensor, shape: torch.Size, what: str, cache: KV8Cache, B: int, packed: bool):

@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import lib as L
-from .kv8 import _call
+from .kv8 import _call, narrowed
 
 _DTYPES = {torch.float32: L.UW_DTYPE_F32, torch.bfloat16: L.UW_DTYPE_BF16}
 _ARGS = Struct("@P2q P2q 5P Pq 4idi4x")        # uw_verify_args
@@ -19,7 +19,7 @@ _ARGS = Struct("@P2q P2q 5P Pq 4idi4x")        # uw_verify_args
 def _ints(x: torch.Tensor, shape, what: str, dev: int) -> torch.Tensor:
     if x.shape != shape or x.dtype not in (torch.int32, torch.int64) or x.get_device() != dev:
         raise ValueError(f"{what} must be int32 {list(shape)} beside target, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+    return x if x.dtype is torch.int32 and x.is_contiguous() else narrowed(x)
 
 
 @lru_cache(maxsize=4096)
