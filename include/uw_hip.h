@@ -231,7 +231,7 @@ int uw_kv8_read(const uw_kv8_store_args* args, void* stream);
 /* Attention of n_heads query heads (a multiple of n_kv_heads; query head h reads kv head h / (n_heads / n_kv_heads)) over the
  * first len[b] cached tokens; with causal != 0 token t of the n tokens of a sequence sees keys 0 .. len[b] - n + t (its own
  * key, appended before, is the last).  o: rows like q; lse (may be NULL) f32 [n_tok][n_heads]: log of the sum of exp(scores).
- * A row that sees no key (len[b] <= 0 among others) gives 0 and lse = -inf.  scale multiplies q.k.  ws: ws_bytes of scratch, at least what
+ * A row that sees no key (len[b] <= 0 among others) gives 0 and lse = -inf.  scale (finite) multiplies q.k.  ws: ws_bytes of scratch, at least what
  * uw_kv8_attention_workspace_bytes() answers for the same arguments (it reads no device memory; -1: arguments refused),
  * 16-byte aligned, not shared by calls that may run at the same time; NULL if that is 0. */
 int64_t uw_kv8_attention_workspace_bytes(const uw_kv8_attention_args* args);

@@ -1,0 +1,28 @@
+"""More of what the 8-bit cache's operators refuse: no GPU is touched."""
+import pytest
+import torch
+
+from whisper_amd import kv8
+from whisper_amd import lib as L
+
+
+def _cache():
+    return kv8.KV8Cache.allocate(4, 2, 64, 16, "int8", device="cpu")
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39, -1e300])
+def test_scales_that_are_no_f32_numbers(scale):
+    c, table, ln = _cache(), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="scale"):
+        kv8.attention(torch.zeros(1, 1, 2, 64), c, table, ln, scale=scale)
+    with pytest.raises(L.UwError, match="GPU"):
+        kv8.attention(torch.zeros(1, 1, 2, 64), c, table, ln, scale=-3.4e38)
+
+
+def test_library_refuses_such_scales_too():
+    lib = L.load()
+    a = (64, 64, 64, 64, 4, 2, 16, 64, L.UW_KV8_INT8, 0, 64, 64, 0, 3, 1, 3, 1, L.UW_DTYPE_BF16, 64, 128, 128, 64, 64, 128, 128, 64, 0, 0, 0, 2, 1)
+    for scale in (float("nan"), float("inf"), -float("inf")):
+        args = kv8._CACHE.pack(*a[:10]) + kv8._ATTEND.pack(*a[10:], scale, 0)
+        assert lib.uw_kv8_attention(args, None) > 0 and b"scale" in lib.uw_last_error()
+        assert lib.uw_kv8_attention_workspace_bytes(args) == -1

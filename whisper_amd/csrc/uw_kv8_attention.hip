@@ -738,6 +738,7 @@ int check_attention(const char* fn, const uw_kv8_attention_args* a)
     RUN(check_seqs(fn, &a->seqs));
     RUN(check_tokens(fn, "q", &a->q, &a->seqs));
     RUN(check_tokens(fn, "o", &a->o, &a->seqs));
+    UW_REQUIRE(fabsf(a->scale) < INFINITY, "%s: scale must be a finite number", fn);
     UW_REQUIRE(a->n_heads > 0 && a->n_heads % a->cache.n_kv_heads == 0, "%s: %d query heads over %d kv heads", fn, a->n_heads, a->cache.n_kv_heads);
     return UW_OK;
 }

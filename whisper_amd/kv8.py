@@ -18,6 +18,7 @@ _FORMAT_OF = {torch.int8: L.UW_KV8_INT8, torch.float8_e4m3fn: L.UW_KV8_E4M3}
 _DTYPES = {torch.float32: L.UW_DTYPE_F32, torch.bfloat16: L.UW_DTYPE_BF16}
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+_F32_MAX = torch.finfo(torch.float32).max
 # the argument structures of the C ABI behind their uw_kv8_cache
 _CACHE = Struct("@4P6i")
 _CACHE_DIMS = Struct("@6i")
@@ -204,6 +205,10 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
     heads, d = shape[-2], cache._d
     if heads % cache._h or heads == 0:
         raise ValueError(f"{heads} query heads over {cache._h} cached heads")
+    if scale is None:
+        scale = d ** -0.5
+    elif not abs(scale) <= _F32_MAX:
+        raise ValueError(f"scale must be a finite f32 number, got {scale}")
     if out is not None and (out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() & 15):
         raise ValueError("out must be contiguous, 16-byte aligned and like q")
     _on_gpu(cache)
@@ -216,5 +221,5 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
     _call(L.load().uw_kv8_attention, cache._c + _ATTEND.pack(
         table.data_ptr(), kv_len.data_ptr(), tok_start.data_ptr() if packed else 0, n, width, B, T, dtype, *cq, out.data_ptr(), T * heads * d,
         heads * d, d, lse.data_ptr() if return_lse else 0, ws.data_ptr() if need else 0, need, heads, 1 if causal else 0,
-        d ** -0.5 if scale is None else float(scale), 0), dev)
+        float(scale), 0), dev)
     return (out, lse) if return_lse else out
