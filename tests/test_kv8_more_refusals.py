@@ -26,3 +26,12 @@ def test_library_refuses_such_scales_too():
         args = kv8._CACHE.pack(*a[:10]) + kv8._ATTEND.pack(*a[10:], scale, 0)
         assert lib.uw_kv8_attention(args, None) > 0 and b"scale" in lib.uw_last_error()
         assert lib.uw_kv8_attention_workspace_bytes(args) == -1
+
+
+def test_the_tensors_of_a_cache_stay():
+    """The operators hold on to the addresses of the tensors that a cache was made of: another tensor in their place would not be what is used."""
+    c = _cache()
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    assert c.k.shape == (4, 2, 16, 64) and c.v.shape == (4, 2, 64, 16) and c.k_scale.shape == c.v_scale.shape == (4, 2)

@@ -29,9 +29,9 @@ _ATTEND = Struct("@3Pq4i P3q P3q 2Pq2ifi")
 
 class KV8Cache:
     """The four tensors of a cache: k [pages, kv heads, page, head_dim] and v [pages, kv heads, head_dim, page] (int8 or
-    float8_e4m3fn), k_scale and v_scale f32 [pages, kv heads]."""
+    float8_e4m3fn), k_scale and v_scale f32 [pages, kv heads].  A cache keeps the tensors it was made of."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "_c", "_dev", "_h", "_d")
+    __slots__ = ("_tensors", "_ks", "_c", "_dev", "_h", "_d")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         dtype = k.dtype
@@ -48,7 +48,7 @@ class KV8Cache:
         dev = k.get_device()
         if v.get_device() != dev or k_scale.get_device() != dev or v_scale.get_device() != dev:
             raise ValueError("cache tensors must be on one device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors, self._ks = (k, v, k_scale, v_scale), k_scale
         self._c = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, h, p, d, fmt, 0)
         self._dev, self._h, self._d = dev, h, d
 
@@ -63,6 +63,10 @@ class KV8Cache:
         return cls(codes[0].view(n_pages, n_kv_heads, page, head_dim), codes[1].view(n_pages, n_kv_heads, head_dim, page),
                    scales[0], scales[1])
 
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
     n_pages = property(lambda self: self.k.shape[0])
     n_kv_heads = property(lambda self: self.k.shape[1])
     page = property(lambda self: self.k.shape[2])
@@ -168,7 +172,7 @@ def read(cache: KV8Cache, table: torch.Tensor, first: torch.Tensor, n_tok: int, 
         tok_start = _index(tok_start, B + 1, "tok_start", dev)
     _on_gpu(cache)
     h, d = cache._h, cache._d
-    k = cache.k_scale.new_empty((n_tok, h, d) if packed else (B, n_tok, h, d), dtype=dtype)
+    k = cache._ks.new_empty((n_tok, h, d) if packed else (B, n_tok, h, d), dtype=dtype)
     v = torch.empty_like(k)
     st = (0, h * d, d) if packed else (n_tok * h * d, h * d, d)
     _call(L.load().uw_kv8_read, cache._c + _STORE.pack(table.data_ptr(), first.data_ptr(), tok_start.data_ptr() if packed else 0,
@@ -215,9 +219,9 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
     n, T = (shape[0], 0) if packed else (B * shape[1], shape[1])
-    lse = cache.k_scale.new_empty((n, heads) if packed else (B, T, heads)) if return_lse else None
+    lse = cache._ks.new_empty((n, heads) if packed else (B, T, heads)) if return_lse else None
     need = _workspace_bytes(cache._c[_ADDRESSES:], n, width, B, T, dtype, packed, heads)
-    ws = cache.k_scale.new_empty(need // 4) if need else None
+    ws = cache._ks.new_empty(need // 4) if need else None
     _call(L.load().uw_kv8_attention, cache._c + _ATTEND.pack(
         table.data_ptr(), kv_len.data_ptr(), tok_start.data_ptr() if packed else 0, n, width, B, T, dtype, *cq, out.data_ptr(), T * heads * d,
         heads * d, d, lse.data_ptr() if return_lse else 0, ws.data_ptr() if need else 0, need, heads, 1 if causal else 0,
