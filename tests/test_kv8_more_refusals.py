@@ -35,3 +35,19 @@ def test_the_tensors_of_a_cache_stay():
         with pytest.raises(AttributeError):
             setattr(c, name, getattr(c, name).clone())
     assert c.k.shape == (4, 2, 16, 64) and c.v.shape == (4, 2, 64, 16) and c.k_scale.shape == c.v_scale.shape == (4, 2)
+
+
+def test_an_output_that_lies_across_the_queries():
+    """Rows that are written while others are still to be read; the queries' own memory, row by row the same, is fine, and so is memory beside it."""
+    c, table, ln = _cache(), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    buf = torch.zeros(3 * 2 * 2 * 64 * 2)
+    q = buf[:768].view(3, 2, 2, 64)
+    for out in (buf[64:832].view(3, 2, 2, 64), buf[704:1472].view(3, 2, 2, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            kv8.attention(q, c, table, ln, out=out)
+    fused = buf.view(3, 2, 2, 128)[..., :64]
+    with pytest.raises(ValueError, match="overlap"):
+        kv8.attention(fused, c, table, ln, out=buf[:768].view(3, 2, 2, 64))
+    for out in (q, buf[768:].view(3, 2, 2, 64)):
+        with pytest.raises(L.UwError, match="GPU"):
+            kv8.attention(q, c, table, ln, out=out)

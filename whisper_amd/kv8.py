@@ -197,7 +197,7 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
     [N, heads, head_dim] with tok_start [B + 1]; heads a multiple of the cache's (grouped heads lie side by side).  causal: the
     last of a sequence's n query tokens sees kv_len[b] keys, the one before one less, and so on; a token that sees none gives 0.
     scale defaults to head_dim ** -0.5 (pass 1.0 for queries scaled before).  Returns the output (in `out`, contiguous and shaped
-    like q, if given) and, with return_lse, f32 log-sum-exp [..., heads].  Rows behind tok_start[B] are not written."""
+    like q, if given; q itself will do) and, with return_lse, f32 log-sum-exp [..., heads].  Rows behind tok_start[B] are not written."""
     B, width = _table(table, cache)
     dev = cache._dev
     kv_len = _index(kv_len, B, "kv_len", dev)
@@ -215,6 +215,10 @@ def attention(q: torch.Tensor, cache: KV8Cache, table: torch.Tensor, kv_len: tor
         raise ValueError(f"scale must be a finite f32 number, got {scale}")
     if out is not None and (out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() & 15):
         raise ValueError("out must be contiguous, 16-byte aligned and like q")
+    if out is not None and out.numel() and not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
+        span = 1 + sum((n - 1) * s for n, s in zip(shape, q.stride()))
+        if q.data_ptr() < out.data_ptr() + out.numel() * q.element_size() and out.data_ptr() < q.data_ptr() + span * q.element_size():
+            raise ValueError("out must not overlap q (but may be q itself, if that is contiguous)")
     _on_gpu(cache)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
