@@ -13,7 +13,7 @@ Z = 0.0
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("T,H,more", [(1, 2, 0), (1, 1, 100), (24, 2, 0), (200, 96, 0)])      # 16 rows; cut and joined; 32 rows; side by side
+@pytest.mark.parametrize("T,H,more", [(1, 2, 0), (1, 1, 100), (24, 2, 0), (200, 112, 0)])      # 16 rows; cut and joined; 32 rows; side by side
 @pytest.mark.parametrize("sizes", [(Z, 1e-5, 1e-5), (1e-5, 1e-6, Z), (1e-3, Z, 1e-9, Z), (Z, 1e-37, 1e-37, Z), (1.0, Z, 1e-37), (Z, 1e30, Z), (Z,) * 4, (Z,)])
 def test_pages_of_zeros(fmt, dtype, T, H, more, sizes):
     g = _gen(T + H + len(sizes))

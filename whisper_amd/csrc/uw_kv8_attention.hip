@@ -752,19 +752,35 @@ struct AttnPlan {
     long groups, ws_bytes;   // items of a head
 };
 
-// How a call is cut.
+// How a call is cut.  (Device times in us of random int8 caches, calls back to back in a graph.)
 //  - up to 16 rows of a kv head: one row tile, the waves share the keys
-//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), where that gives a workgroup to each of the 256 CUs,
-//    with 64 channels to one and a half times as many; else tiles of 16 or 32 rows whose four waves share the keys -- more workgroups
-//    for the same rows.  Measured (us, side by side / tiles of 32 / tiles of 16; bf16, workgroups of the first): 64 channels, 170 rows
-//    over 1500 keys: 128: 31.0 / 21.2 / 20.7, 256: 31.1 / 27.7 / 32.2, 384: 42.2 / 44.7 / 56.3, 512: 42.9 / 58.8 / 74.5; 2048 causal rows
-//    over 4096 keys: 256: 74.1 / 68.2 / 91.5, 384: 95.2 / 97.5 / 127; 33380 causal rows of 4 heads over 5000 keys 151 / 225 / 296.
-//    128 channels, 2048 causal rows over 8192 keys: 128: 198 / 122 / 211, 192: 199 / 184 / 325, 256: 199 / 242 / 445.
-//    Tiles of 16 where 64-channel rows are few, 12800 of all heads, or f32: 10880 rows over 1500 keys 20.4 / 21.2 (32 rows), 16320 29.0 /
-//    26.5, 2720 10.3 / 14.7; f32 10880 32.0 / 36.1, 19040 43.6 / 48.0.  (Rows of 128 channels make too little of a key's many bytes.)
+//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), where that gives 448 workgroups, with 128 channels 320;
+//    else tiles of 16 or 32 rows whose four waves share the keys -- more workgroups for the same rows, each converting the codes for itself.
+//    Measured (side by side / tiles of 32 / tiles of 16; workgroups of the first):
+//      bf16  64 channels  170 rows over 1500 keys        128: 40 / 22.6 / 21.1   256: 40 / 30.9 / 35.5   384: 54 / 47 / 54   448: 54 / 56 / 64   512: 55 / 61 / 76
+//                         2048 causal rows over 4096     256: 97 / 67 / 82   384: 103 / 94 / 118   448: 106 / 111 / 144   512: 109 / 120 / 155
+//                         33380 causal rows of 4 heads over 5000   190 / 257 / 325
+//           128 channels  2048 causal rows over 8192     128: 254 / 122 / 166   256: 255 / 227 / 344   320: 309 / 323 / 546   384: 318 / 361 / 605
+//                         170 rows over 1500             256: 55 / 54 / 80   320: 76 / 74 / 100   384: 76 / 90 / 131
+//      f32   64 channels  170 rows over 1500             128: 48 / 28.2 / 24.7   384: 74 / 63 / 67   448: 75 / 75.5 / 81   512: 76 / 81 / 96
+//                         2048 causal rows over 4096     256: 122 / 84 / 95   384: 146 / 124 / 142   448: 150 / 151 / 183
+//           128 channels  2048 causal rows over 4096     256: 124 / - / 92   320: 135 / - / 129   384: 137 / - / 145   448: 138 / - / 197
+//                         170 rows over 1500             240: 52 / - / 56   336: 68 / - / 79
+//    Tiles of 16 where 64-channel rows are few, 12800 of all heads, f32 25600: 2720 rows over 1500 keys 10.6 / 14.9 (32 rows), 10880 21.1 /
+//    22.6, 16320 30.2 / 28.8; f32 10880 24.7 / 28.2, 19040 36.8 / 39.0, 27200 52 / 51, 32640 67 / 63.  (Rows of 128 channels make too little
+//    of a key's many bytes.)
 //  - long sequences are cut further where the waves share the keys, into items of equal size (chunk_of), joined by a second launch.
-//    Short ones are not: up to 32 blocks, eight or four waves are through sooner than a second launch is.  Nor are many: 512 tables of
-//    up to 64 blocks, or 4096 of any length, fill the chip evenly enough as they are
+//    Short ones are not: up to 32 blocks (33 where the table's last one is counted) eight waves are through as soon as a second launch is --
+//    one token of 8 heads over 2048 keys 11.1 either way, over 2300 12.1 uncut and 11.4 cut, over 4000 18.1 and 11.7.  Nor are many: 512
+//    tables of up to 64 blocks (2300 keys 25.6 uncut, 29.2 cut; 4000 43 and 46; ragged to 4000 33 and 37), or 4096 of any length (over 2300 183
+//    and 189, over 4500 358 and 363, ragged to 8000 655 and 660).  Between these bounds the cut is worth most where the lengths are long and
+//    few, and costs up to a quarter where workgroups are many already (256 over 4000 keys: 23 uncut, 30 cut).
+//    At least half of the 512 items wanted are cut pieces, however many tiles there are: a quarter, half, three quarters, all: five tokens of 8
+//    kv heads of 128 channels over 8 x 32768 keys 109 / 108 / 108 / 100, 60 x 8 over 8192 165 / 162 / 162 / 247.
+//  - eight waves instead of four for up to 256 workgroups that are not cut: over 1500 keys 6 workgroups 10.6 / 11.5, f32 11.6 / 12.5; 256 11.6 /
+//    13.2, f32 12.9 / 14.2; 320 16.9 / 16.7, f32 22.0 / 18.6; 1024 33.8 / 33.6, f32 45 / 35
+//  The bounds on blocks go by the table's width, for lengths are known on the device only: under a table for 32768 tokens one window of 6 heads
+//  takes 11.5 instead of 9.7, 32 ragged sequences of up to 448 tokens 10.6 instead of 7.2.
 AttnPlan plan_attention(const uw_kv8_attention_args* a)
 {
     AttnPlan p;
@@ -778,10 +794,10 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     p.wr = 1;
     if (rows > 32) {
         const long heads = (long)B * c->n_kv_heads;
-        if (ceil_div(rows, 64 * p.rt) * heads >= (c->head_dim == 64 ? 384 : 256)) {
+        if (ceil_div(rows, 64 * p.rt) * heads >= (c->head_dim == 64 ? 448 : 320)) {
             p.wk = 1;
             p.wr = 4;
-        } else if (c->head_dim == 64 && (a->seqs.dtype == UW_DTYPE_F32 || rows * heads < 12800)) {
+        } else if (c->head_dim == 64 && rows * heads < (a->seqs.dtype == UW_DTYPE_F32 ? 25600 : 12800)) {
             p.rt = 1;
         }
     }
