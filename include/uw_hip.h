@@ -223,10 +223,10 @@ typedef struct uw_kv8_attention_args {
  * next to 1/127, 2^-126 at least; e4m3: the smallest power of two that leaves codes up to 448); otherwise the scale
  * stays while the new values fit and grows by a power of two if not, the earlier tokens' codes being re-rounded.  A NaN or
  * infinity makes the scale of its block and head NaN until the block is begun again: whatever reads that block gives NaN.
- * A block must not be touched by two sequences of one call (shared prefixes end on a page boundary).  Codes behind the last
+ * A page must not be touched twice by one call, from two sequences or two blocks of one (shared prefixes end on a page boundary).  Codes behind the last
  * token are left as they are. */
 int uw_kv8_append(const uw_kv8_store_args* args, void* stream);
-/* Reads tokens back as values (code * scale, rounded once to dtype): positions len[b], len[b] + 1, ... into k and v. */
+/* Reads tokens back as values (code * scale in f32, that rounded to dtype): positions len[b], len[b] + 1, ... into k and v. */
 int uw_kv8_read(const uw_kv8_store_args* args, void* stream);
 /* Attention of n_heads query heads (a multiple of n_kv_heads; query head h reads kv head h / (n_heads / n_kv_heads)) over the
  * first len[b] cached tokens; with causal != 0 token t of the n tokens of a sequence sees keys 0 .. len[b] - n + t (its own
@@ -246,7 +246,7 @@ int uw_kv8_attention(const uw_kv8_attention_args* args, void* stream);
  * 1.1e-12 at most.  temperature 0: a token is accepted while it
  * is its row's arg-max (the lowest index of equal ones) and the next token is the arg-max; draft and uniforms are not read.
  * accepted i32 [B]; tokens i32 [B][N+1]: the accepted tokens, the next token, then -1.  The next token is -1 if its row holds
- * a NaN or has no mass (the decoder-run failure of core.py:948-956); a drafted id outside 0..V-1 is never accepted.
+ * a NaN or has no mass -- at temperature 0 a NaN only -- (the decoder-run failure of core.py:948-956); a drafted id outside 0..V-1 is never accepted.
  * ws: ws_bytes of scratch, at least uw_verify_draft_workspace_bytes() (-1: arguments refused), 16-byte aligned, not shared by
  * calls that may run at the same time. */
 typedef struct uw_verify_args {

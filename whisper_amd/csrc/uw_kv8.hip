@@ -16,8 +16,9 @@ __device__ __forceinline__ int touched(int pos, int n, int log2P)
 // Append and read: a workgroup per touched block, head and half, TPB threads (64 for a few tokens, so that a decode step's tokens do
 // not each hold four waves).  Both are bound by memory: values once, codes once, nothing between.  V passes through LDS on its way to
 // or from [D][P], a channel's tokens at a pitch of P + 4 bytes, so that the words of a wave fall into different banks.
-// Measured: 32 x 1500 tokens of 12 heads of 64, bf16 (221 MB each way) stored in 53 us, 4.2 TB/s, read back in 44, 5.0 TB/s (a large copy:
-// 4.65); the newest token of 128 sequences stored in 7.8 us, which is one chain of length, page, value and scale, not bandwidth (0.6 MB).
+// Measured, calls back to back in a graph: 32 x 1500 tokens of 12 heads of 64, bf16 (221 MB each way) stored in 51.5 us, 4.3 TB/s, read back in
+// 42.4, 5.2 TB/s (a large copy: 4.65); the newest token of 128 sequences stored in 6.7 us, which is one chain of length, page, value and
+// scale, not bandwidth (0.6 MB).
 
 struct Block {           // one block of a call
     int b, r0, rows;            // sequence, first row in the block, rows of the call
@@ -324,8 +325,9 @@ int check_store(const char* fn, const uw_kv8_store_args* a)
 }
 
 // One wave per block and head for a decode step's tokens, two otherwise: most of a workgroup's life is waiting for its lengths, its
-// page and its values, so many small ones beat few large ones (128 sequences' newest token: 7.0 us with one wave, 8.4 with two, 10.5
-// with four; 32 x 1500 tokens read back: 44, 38 and 48 us).
+// page and its values, so many small ones beat few large ones.  One wave / two, back to back in a graph: 128 sequences' newest token stored 6.7 /
+// 7.6 us, their last blocks read back 9.4 / 9.8; 32 x 1500 tokens stored 55.7 / 51.5, read back 43.2 / 42.4; 16 x up to 701 f32 tokens of 128
+// channels stored 22.1 / 17.4.
 bool few_tokens(const uw_kv8_store_args* a)
 {
     const long per = a->seqs.tok_start ? ceil_div(a->seqs.n_tok, a->seqs.B) : a->seqs.T;

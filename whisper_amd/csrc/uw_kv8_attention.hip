@@ -18,17 +18,17 @@ namespace {
 //
 // bf16 queries enter exactly, their weights as two bf16 planes: off by 2^-16 of each at most, with the whole of f32's exponent, so that
 // a row has its result to the same error when its largest weights meet values of zero.  (One f16 plane, which is faster -- 145 us for the
-// prompts below when this took 184, no difference where the stream of codes bounds -- loses the weights below 2^-25 of the largest and keeps
-// them in the sum.)  f32 queries and weights enter as three planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a
+// prompts below when this took 185, 2 to 4 % where the stream of codes bounds, 0.6 of 9.7 us for one window -- loses the weights below 2^-25 of the
+// largest and keeps them in the sum.)  f32 queries and weights enter as three planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a
 // third of the bf16 rate.
 //
-// What bounds it: few rows of a head -- the stream of codes; 128 windows' token over 1500 keys of 12 heads (296 MB) 48.8 us, 6.1 TB/s; five
-// tokens of 4 heads a kv head over long ragged tables (297 MB) 57.7 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
-// which has a multiply-add, an exponential (a quarter of the rate), an addition and the two planes to do for each weight, and the matrix
-// unit, with 192 or 384 multiply-adds for it: 33380 causal rows of 4 heads over 5000 keys 184 us, 590 TFLOP/s counted as 4 D
-// operations a weight.  One window of 6 heads -- a chain of lengths, pages, codes, three blocks a wave and the join of eight waves: 8.9 us
-// (e4m3 7.4; int8's conversions are the rest).  170 f32 rows of 64 heads over 1500 keys: 24.3 us, 170 TFLOP/s, three times that on the
-// matrix unit.
+// What bounds it: few rows of a head -- the stream of codes; 128 windows' token over 1500 keys of 12 heads, e4m3 (296 MB) 49.6 us, 6.0 TB/s;
+// five tokens of 4 heads a kv head over long ragged tables (297 MB) 58 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
+// which has a multiply-add, an exponential (a quarter of the rate), an addition and the two planes to do for each weight; it is at work in 72 %
+// of the cycles, the matrix unit, with 192 or 384 multiply-adds for a weight, in 39 %, and LDS in 40 %, without bank conflicts: 33380 causal
+// rows of 4 heads over 5000 keys 185 us, 585 TFLOP/s counted as 4 D operations a weight.  One window of 6 heads -- a chain of lengths, pages,
+// codes, three blocks a wave and the join of eight waves: 9.7 us (e4m3 9.2).  170 f32 rows of 64 heads over 1500 keys: 24.4 us, 171
+// TFLOP/s, three times that on the matrix unit.
 //
 // What a decoder step adds: one query token per window, its output in the operand layout of the product that follows, and the
 // probabilities of the alignment heads.
@@ -136,7 +136,8 @@ __device__ __forceinline__ int chunk_of(const AttnArgs& p, int rows)
 }
 __device__ __forceinline__ int splits_of(const AttnArgs& p, int b, int chunk) { return max(1, (blocks_of(p, b) + chunk - 1) / chunk); }
 
-// a 16-byte piece of the cache; ONCE: no other workgroup will want it, so it need not stay in L2
+// a 16-byte piece of the cache; ONCE: it need not stay in L2.  The shapes whose waves share the keys ask so: with one row tile of a head no
+// other workgroup wants the piece.  With several they do, and ask again; what the hint does there has not been measured apart.
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 template <bool ONCE> __device__ __forceinline__ uint4 ld_codes(const void* p)
 {
@@ -224,7 +225,8 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 
     // which kv head, sequence, rows and part of the keys.  Heads run fastest: a head's workgroups land on one XCD when their number
     // is a multiple of 8, and share its L2.  The last rows of all sequences come first: causal ones see most, and a long item that
-    // starts late is waited for (4500, 2782 and 1063 tokens of 16 heads: 187 us in the sequences' order, 156 so).
+    // starts late is waited for (4500, 2782 and 1063 tokens of 16 heads, with one f16
+    // plane of weights: 187 us in the sequences' order, 156 so).
     int b, tile, split = 0, splits = 1, chunk = 0;
     const int kvh = blockIdx.x % c.Hkv, item = blockIdx.x / c.Hkv;
     if (p.n_split > 1) {
@@ -757,7 +759,8 @@ struct AttnPlan {
 //  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), where that gives 448 workgroups, with 128 channels 320;
 //    else tiles of 16 or 32 rows whose four waves share the keys -- more workgroups for the same rows, each converting the codes for itself.
 //    Measured (side by side / tiles of 32 / tiles of 16; workgroups of the first):
-//      bf16  64 channels  170 rows over 1500 keys        128: 40 / 22.6 / 21.1   256: 40 / 30.9 / 35.5   384: 54 / 47 / 54   448: 54 / 56 / 64   512: 55 / 61 / 76
+//      bf16  64 channels  170 rows over 1500 keys        128: 40 / 22.6 / 21.1   256: 40 / 30.9 / 35.5   384: 54 / 47 / 54   448: 54 / 56 / 64
+//                                                        512: 55 / 61 / 76
 //                         2048 causal rows over 4096     256: 97 / 67 / 82   384: 103 / 94 / 118   448: 106 / 111 / 144   512: 109 / 120 / 155
 //                         33380 causal rows of 4 heads over 5000   190 / 257 / 325
 //           128 channels  2048 causal rows over 8192     128: 254 / 122 / 166   256: 255 / 227 / 344   320: 309 / 323 / 546   384: 318 / 361 / 605

@@ -12,10 +12,11 @@
 // in L2 or the Infinity Cache by then); (3) a workgroup per sequence finds the chunk, then the token in it.  Probabilities need no
 // (1), logits without a draft no (2); greedy verification needs the arg-max of (1) and then one small launch.
 //
-// Measured: 64 windows of nought to five tokens, both models' f32 logits (V 51865, 80 MB read): 21.1 + 13.4 + 7.6 us.  (1) does as much f64
-// arithmetic as reading, 3.8 TB/s; (2) and (3) are chains of statistics, decision, scores and sums with few rows left to work side by side.
-// One window of four tokens 3.7 + 8.8 us.  Greedy, 128 windows of four tokens, bf16 (66 MB): 15.9 + 3.9 us, 4.2 TB/s.  Chunks of 2048 scores
-// took 26.4 + 14.2 + 7.7 us and greedy 24.2, of 8192 23.4 + 16.6 + 13.4 and 17.5, when these took 22.7 + 14.1 + 8.6 and 17.8.
+// Measured: 64 windows of nought to five tokens, both models' f32 logits (V 51865, 80 MB read): 20.6 + 13.0 + 6.9 us by kernel trace, 41 in
+// a row of calls.  (1) does as much f64 arithmetic as reading, 3.9 TB/s; (2) and (3) are chains of statistics, decision, scores and sums
+// with few rows left to work side by side.  One window of four tokens 3.5 + 9.0 us.  Greedy, 128 windows of four tokens, bf16 (66 MB): 15.5 +
+// 4.0 us, 4.3 TB/s.  Probabilities of both models, five tokens: 64 windows (26.5 MB, no (1)) 12.8 us, one 9.5.  Chunks of 2048 scores took
+// 26.4 + 14.2 + 7.7 us and greedy 24.2, of 8192 23.4 + 16.6 + 13.4 and 17.5, when these took 22.7 + 14.1 + 8.6 and 17.8.
 #include "../../include/uw_hip.h"
 #include "uw_common.h"
 #include "uw_kernels.h"

@@ -44,7 +44,8 @@ def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: Optional
     arg-max of its row; uniforms and draft are not used.
 
     Returns accepted i32 [B] and tokens i32 [B, N + 1]: the accepted tokens, then the next token, then -1.  The tokens are
-    distributed as if drawn from the target alone.  A next token of -1 says that its row held a NaN or no mass."""
+    distributed as if drawn from the target alone.  A next token of -1 says that its row held a NaN or no mass
+    (greedy: a NaN)."""
     shape = target.shape
     if len(shape) != 3 or target.dtype not in _DTYPES:
         raise ValueError(f"target must be float32 or bfloat16 [B, N + 1, V], got {target.dtype} {tuple(shape)}")
