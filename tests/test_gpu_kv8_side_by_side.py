@@ -1,6 +1,6 @@
-"""Attention over the 8-bit cache in calls that fill the chip with 128 (64) rows a workgroup, 448 of them and more with 64 channels, 320 with 128:
-many rows, ragged rows, V blocks of very different size, one weight beside thousands, poisoned and missing pages.  References and tolerances
-are those of the tests of the same names."""
+"""Attention over the 8-bit cache in calls that fill the chip with 128 (64) rows a workgroup, at least 448 of them with 64 channels, 320 with
+128: many rows, ragged rows, V blocks of very different size, one weight beside thousands, poisoned and missing pages.  References and
+tolerances are those of the tests of the same names."""
 import pytest
 import torch
 

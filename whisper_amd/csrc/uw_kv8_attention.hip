@@ -18,9 +18,9 @@ namespace {
 //
 // bf16 queries enter exactly, their weights as two bf16 planes: off by 2^-16 of each at most, with the whole of f32's exponent, so that
 // a row has its result to the same error when its largest weights meet values of zero.  (One f16 plane, which is faster -- 145 us for the
-// prompts below when this took 185, 2 to 4 % where the stream of codes bounds, 0.6 of 9.7 us for one window -- loses the weights below 2^-25 of the
-// largest and keeps them in the sum.)  f32 queries and weights enter as three planes (24 bits): the codes being exact in bf16, that is f32 arithmetic at a
-// third of the bf16 rate.
+// prompts below when this took 185, 2 to 4 % where the stream of codes bounds, 0.6 of 9.7 us for one window -- loses the weights below 2^-25
+// of the largest and keeps them in the sum.)  f32 queries and weights enter as three planes (24 bits): the codes being exact in bf16, that
+// is f32 arithmetic at a third of the bf16 rate.
 //
 // What bounds it: few rows of a head -- the stream of codes; 128 windows' token over 1500 keys of 12 heads, e4m3 (296 MB) 49.6 us, 6.0 TB/s;
 // five tokens of 4 heads a kv head over long ragged tables (297 MB) 58 us, 5.1 TB/s, and 4.8 us for the join.  Many rows -- the vector ALU,
@@ -225,8 +225,7 @@ __global__ __launch_bounds__(64 * WK * WR, (sizeof(T) == 2 && D == 64) ? (RT == 
 
     // which kv head, sequence, rows and part of the keys.  Heads run fastest: a head's workgroups land on one XCD when their number
     // is a multiple of 8, and share its L2.  The last rows of all sequences come first: causal ones see most, and a long item that
-    // starts late is waited for (4500, 2782 and 1063 tokens of 16 heads, with one f16
-    // plane of weights: 187 us in the sequences' order, 156 so).
+    // starts late is waited for (4500, 2782 and 1063 tokens of 16 heads, with one f16 plane of weights: 187 us in the sequences' order, 156 so).
     int b, tile, split = 0, splits = 1, chunk = 0;
     const int kvh = blockIdx.x % c.Hkv, item = blockIdx.x / c.Hkv;
     if (p.n_split > 1) {
@@ -756,7 +755,7 @@ struct AttnPlan {
 
 // How a call is cut.  (Device times in us of random int8 caches, calls back to back in a graph.)
 //  - up to 16 rows of a kv head: one row tile, the waves share the keys
-//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), where that gives 448 workgroups, with 128 channels 320;
+//  - more: four waves of rows side by side (128 rows, f32 with 128 channels 64), where that gives 384 workgroups, with 128 channels 256;
 //    else tiles of 16 or 32 rows whose four waves share the keys -- more workgroups for the same rows, each converting the codes for itself.
 //    Measured (side by side / tiles of 32 / tiles of 16; workgroups of the first):
 //      bf16  64 channels  170 rows over 1500 keys        128: 40 / 22.6 / 21.1   256: 40 / 30.9 / 35.5   384: 54 / 47 / 54   448: 54 / 56 / 64
@@ -769,6 +768,10 @@ struct AttnPlan {
 //                         2048 causal rows over 4096     256: 122 / 84 / 95   384: 146 / 124 / 142   448: 150 / 151 / 183
 //           128 channels  2048 causal rows over 4096     256: 124 / - / 92   320: 135 / - / 129   384: 137 / - / 145   448: 138 / - / 197
 //                         170 rows over 1500             240: 52 / - / 56   336: 68 / - / 79
+//    Where the sides cross depends on how full the last tile of a head is and on how long the keys are: of 191 calls drawn at random (160 to
+//    660 workgroups, 64 to 3000 tokens, up to 8000 keys) side by side is the faster one from 264 workgroups on in some and from 620 in others.
+//    These bounds lose 1.8 % against the better side on average (bf16, 64 channels; 320: 3.3, 448: 2.3, 512: 4.1), 3.5 % (bf16, 128; 192: 2.6,
+//    320: 3.8, 384: 8.1), 5.1 % (f32, 64; 320: 7.0, 448: 4.8) and 3.6 % (f32, 128; 192: 0.8, 320: 3.6, 384: 8.1).
 //    Tiles of 16 where 64-channel rows are few, 12800 of all heads, f32 25600: 2720 rows over 1500 keys 10.6 / 14.9 (32 rows), 10880 21.1 /
 //    22.6, 16320 30.2 / 28.8; f32 10880 24.7 / 28.2, 19040 36.8 / 39.0, 27200 52 / 51, 32640 67 / 63.  (Rows of 128 channels make too little
 //    of a key's many bytes.)
@@ -797,7 +800,7 @@ AttnPlan plan_attention(const uw_kv8_attention_args* a)
     p.wr = 1;
     if (rows > 32) {
         const long heads = (long)B * c->n_kv_heads;
-        if (ceil_div(rows, 64 * p.rt) * heads >= (c->head_dim == 64 ? 448 : 320)) {
+        if (ceil_div(rows, 64 * p.rt) * heads >= (c->head_dim == 64 ? 384 : 256)) {
             p.wk = 1;
             p.wr = 4;
         } else if (c->head_dim == 64 && rows * heads < (a->seqs.dtype == UW_DTYPE_F32 ? 25600 : 12800)) {
